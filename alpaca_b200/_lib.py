@@ -131,6 +131,123 @@ class ProjDesc(ctypes.Structure):
     ]
 
 
+class CacheKind(IntEnum):
+    F32 = 0
+    F16 = 1
+    KV4 = 2
+
+
+class Kv4CacheDesc(ctypes.Structure):
+    """alpaca_kv4_cache (include/alpaca_cuda.h)."""
+    _fields_ = [
+        ("k_codes", ctypes.c_void_p),
+        ("v_codes", ctypes.c_void_p),
+        ("k_scales", ctypes.c_void_p),
+        ("v_scales", ctypes.c_void_p),
+        ("code_head_stride", ctypes.c_int64),
+        ("code_unit_stride", ctypes.c_int64),
+        ("scale_head_stride", ctypes.c_int64),
+        ("scale_unit_stride", ctypes.c_int64),
+        ("rows", ctypes.c_int32),
+        ("max_blocks", ctypes.c_int32),
+        ("block_table", ctypes.c_void_p),
+        ("pool_blocks", ctypes.c_int32),
+        ("reserved0", ctypes.c_int32),
+    ]
+
+
+class QkvDesc(ctypes.Structure):
+    """alpaca_qkv_desc (include/alpaca_cuda.h)."""
+    _fields_ = [
+        ("n_seqs", ctypes.c_int32),
+        ("n_heads", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("tokens", ctypes.c_int32),
+        ("start_position", ctypes.c_int32),
+        ("positions", ctypes.c_void_p),
+        ("theta", ctypes.c_float),
+        ("eps", ctypes.c_float),
+        ("interleaved", ctypes.c_int32),
+        ("in_dtype", ctypes.c_int32),
+        ("q_out_dtype", ctypes.c_int32),
+        ("cache_kind", ctypes.c_int32),
+        ("q_norm", ctypes.c_void_p),
+        ("k_norm", ctypes.c_void_p),
+        ("q", ctypes.c_void_p),
+        ("q_token_stride", ctypes.c_int64),
+        ("q_seq_stride", ctypes.c_int64),
+        ("q_out", ctypes.c_void_p),
+        ("q_out_token_stride", ctypes.c_int64),
+        ("q_out_seq_stride", ctypes.c_int64),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("kv_token_stride", ctypes.c_int64),
+        ("kv_seq_stride", ctypes.c_int64),
+        ("k_cache", ctypes.c_void_p),
+        ("v_cache", ctypes.c_void_p),
+        ("cache_row_stride", ctypes.c_int64),
+        ("cache_seq_stride", ctypes.c_int64),
+        ("block_table", ctypes.c_void_p),
+        ("block_stride", ctypes.c_int64),
+        ("block_rows", ctypes.c_int32),
+        ("max_blocks", ctypes.c_int32),
+        ("pool_blocks", ctypes.c_int32),
+        ("cache_rows", ctypes.c_int32),
+        ("kv4", Kv4CacheDesc),
+        ("flags", ctypes.c_uint32),
+        ("reserved0", ctypes.c_uint32),
+    ]
+
+
+class Kv4ReadDesc(ctypes.Structure):
+    """alpaca_kv4_read_desc (include/alpaca_cuda.h)."""
+    _fields_ = [
+        ("n_seqs", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("n_rows", ctypes.c_int32),
+        ("start_row", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("row_starts", ctypes.c_void_p),
+        ("cache", Kv4CacheDesc),
+        ("k_out", ctypes.c_void_p),
+        ("v_out", ctypes.c_void_p),
+        ("out_row_stride", ctypes.c_int64),
+        ("out_seq_stride", ctypes.c_int64),
+        ("flags", ctypes.c_uint32),
+        ("reserved0", ctypes.c_uint32),
+    ]
+
+
+class Kv4AttnDesc(ctypes.Structure):
+    """alpaca_kv4_attn_desc (include/alpaca_cuda.h)."""
+    _fields_ = [
+        ("n_seqs", ctypes.c_int32),
+        ("n_heads", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("tokens", ctypes.c_int32),
+        ("start_position", ctypes.c_int32),
+        ("ctx_lens", ctypes.c_void_p),
+        ("max_ctx_len", ctypes.c_int32),
+        ("q_dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("flags", ctypes.c_uint32),
+        ("q", ctypes.c_void_p),
+        ("q_token_stride", ctypes.c_int64),
+        ("q_seq_stride", ctypes.c_int64),
+        ("out", ctypes.c_void_p),
+        ("out_token_stride", ctypes.c_int64),
+        ("out_seq_stride", ctypes.c_int64),
+        ("scale", ctypes.c_float),
+        ("total_tokens", ctypes.c_int32),
+        ("q_offsets", ctypes.c_void_p),
+        ("start_positions", ctypes.c_void_p),
+        ("cache", Kv4CacheDesc),
+    ]
+
+
 class WeightFormat(IntEnum):
     F16 = 0
     Q8_0 = 1
@@ -153,6 +270,11 @@ EXPORTED_SYMBOLS = (
     "alpaca_cuda_version",
     "alpaca_rope_kv_append",
     "alpaca_decode_project",
+    "alpaca_qkv_append",
+    "alpaca_kv4_read",
+    "alpaca_kv4_attention",
+    "alpaca_kv4_workspace_bytes",
+    "alpaca_kv4_select",
 )
 
 _lib: ctypes.CDLL | None = None
@@ -194,6 +316,17 @@ def load() -> ctypes.CDLL:
     L.alpaca_attn_decode_rope.restype = ctypes.c_int
     L.alpaca_attn_decode_rope.argtypes = [P, ctypes.POINTER(RopeDesc), ctypes.c_void_p, ctypes.c_size_t,
                                           ctypes.c_void_p]
+    L.alpaca_qkv_append.restype = ctypes.c_int
+    L.alpaca_qkv_append.argtypes = [ctypes.POINTER(QkvDesc), ctypes.c_void_p]
+    L.alpaca_kv4_read.restype = ctypes.c_int
+    L.alpaca_kv4_read.argtypes = [ctypes.POINTER(Kv4ReadDesc), ctypes.c_void_p]
+    L.alpaca_kv4_attention.restype = ctypes.c_int
+    L.alpaca_kv4_attention.argtypes = [ctypes.POINTER(Kv4AttnDesc), ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t,
+                                       ctypes.c_void_p]
+    L.alpaca_kv4_workspace_bytes.restype = ctypes.c_int
+    L.alpaca_kv4_workspace_bytes.argtypes = [ctypes.POINTER(Kv4AttnDesc), ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]
+    L.alpaca_kv4_select.restype = ctypes.c_int
+    L.alpaca_kv4_select.argtypes = [ctypes.POINTER(Kv4AttnDesc), ctypes.POINTER(ctypes.c_int)]
     _lib = L
     return L
 

@@ -17,8 +17,9 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libalpaca_cuda.so"
-SOURCES = ["api.cu", "attn_decode.cu", "attn_general.cu", "attn_prefill_sm100.cu", "rope_kv.cu", "decode_proj.cu"]
-HEADERS = ["common.cuh", "internal.h"]
+SOURCES = ["api.cu", "attn_decode.cu", "attn_general.cu", "attn_prefill_sm100.cu", "rope_kv.cu", "decode_proj.cu",
+           "kv4_cache.cu", "attn_kv4.cu"]
+HEADERS = ["common.cuh", "internal.h", "kv4.cuh"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CFLAGS = ["-O3", "-std=c++17", "-lineinfo", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",

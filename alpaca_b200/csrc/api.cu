@@ -348,6 +348,196 @@ alpaca_cuda_status run(const alpaca_attn_desc* dp, alpaca_attn_kernel kind, void
     return launched(e, "attention");
 }
 
+// ---- 4-bit cache entry points
+
+// Layout checks of a 4-bit cache that `seqs` sequences use up to row `rows_needed` (host-known bound; 0: none known).
+alpaca_cuda_status validate_kv4_cache(const alpaca_kv4_cache& c, int n_seqs, int n_kv_heads, int head_dim, int64_t rows_needed,
+                                      const char* who) {
+    auto bad = [&](const char* what) {
+        char sh[200];
+        std::snprintf(sh, sizeof(sh), "%s: 4-bit cache: %s (rows=%d max_blocks=%d pool=%d Hkv=%d d=%d)", who, what, c.rows,
+                      c.max_blocks, c.pool_blocks, n_kv_heads, head_dim);
+        return fail(ALPACA_CUDA_ERR_INVALID_ARGUMENT, sh);
+    };
+    if (!c.k_codes || !c.v_codes || !c.k_scales || !c.v_scales) return bad("null pointer");
+    if (!aligned16(c.k_codes) || !aligned16(c.v_codes) || !aligned16(c.k_scales) || !aligned16(c.v_scales))
+        return bad("pointers must be 16-byte aligned");
+    if (c.rows < 16 || c.rows % 16) return bad("rows must be a positive multiple of 16");
+    if (c.code_head_stride % 16 || c.code_unit_stride % 16 || c.scale_head_stride % 8 || c.scale_unit_stride % 8)
+        return bad("strides must be multiples of 16 bytes");
+    const int64_t code_rows = static_cast<int64_t>(c.rows) * (head_dim / 2), scale_rows = static_cast<int64_t>(c.rows) * (head_dim / 32);
+    if (n_kv_heads > 1 && (c.code_head_stride < code_rows || c.scale_head_stride < scale_rows))
+        return bad("head strides smaller than a head's rows");
+    const int64_t units = c.block_table ? c.pool_blocks : n_seqs;
+    if (c.code_unit_stride < 0 || c.scale_unit_stride < 0 ||
+        (units > 1 && (c.code_unit_stride < code_rows || c.scale_unit_stride < scale_rows)))
+        return bad("unit strides smaller than a head's rows");
+    if (c.block_table) {
+        if (c.max_blocks < 1 || c.pool_blocks < 1) return bad("a paged cache needs max_blocks and pool_blocks >= 1");
+        if (rows_needed > static_cast<int64_t>(c.max_blocks) * c.rows) return bad("block table too short for the rows asked");
+    } else if (rows_needed > c.rows) {
+        return bad("rows past the cache");
+    }
+    return ok();
+}
+
+bool kv4_head_dim_ok(int d) { return d >= 32 && d <= 256 && d % 32 == 0; }
+bool dtype_ok(int t) { return t == ALPACA_F32 || t == ALPACA_F16; }
+
+alpaca_cuda_status validate_qkv(const alpaca_qkv_desc* dp) {
+    if (!dp) return fail(ALPACA_CUDA_ERR_INVALID_ARGUMENT, "qkv: null descriptor");
+    const alpaca_qkv_desc& d = *dp;
+    auto bad = [&](const char* what) {
+        char sh[240];
+        std::snprintf(sh, sizeof(sh), "qkv: %s: seqs=%d T=%d start=%d H=%d/%d d=%d", what, d.n_seqs, d.tokens, d.start_position,
+                      d.n_heads, d.n_kv_heads, d.head_dim);
+        return fail(ALPACA_CUDA_ERR_INVALID_ARGUMENT, sh);
+    };
+    if (d.n_seqs < 1 || d.n_seqs > 65535 || d.tokens < 1 || d.n_heads < 0 || d.n_kv_heads < 0 || d.start_position < 0 ||
+        (d.n_heads == 0 && d.n_kv_heads == 0) || d.n_heads > (1 << 20) || d.n_kv_heads > (1 << 20))
+        return bad("shapes");
+    if (!kv4_head_dim_ok(d.head_dim)) return bad("headDim must be a multiple of 32 up to 256");
+    if (!(d.theta > 0.f) || !std::isfinite(d.theta)) return bad("theta must be finite and > 0");
+    if (d.interleaved != 0 && d.interleaved != 1) return bad("interleaved must be 0 or 1");
+    if (d.flags != 0) return bad("unknown flags");
+    if (!dtype_ok(d.in_dtype) || (d.n_heads > 0 && !dtype_ok(d.q_out_dtype))) return bad("unknown dtype");
+    if (d.start_position > (1 << 30) || d.tokens > (1 << 30) - d.start_position) return bad("positions out of range");
+    if ((d.q_norm || d.k_norm) && (!(d.eps > 0.f) || !std::isfinite(d.eps))) return bad("eps must be finite and > 0");
+    if (!aligned16(d.q_norm) || !aligned16(d.k_norm)) return bad("norm weights must be 16-byte aligned");
+    const int64_t is = static_cast<int64_t>(dtype_size(d.in_dtype));
+    if (d.n_heads > 0) {
+        const int64_t hq = static_cast<int64_t>(d.n_heads) * d.head_dim, os = static_cast<int64_t>(dtype_size(d.q_out_dtype));
+        if (!d.q || !d.q_out || !aligned16(d.q) || !aligned16(d.q_out)) return bad("q / q_out null or not 16-byte aligned");
+        if (d.q_token_stride < hq || d.q_out_token_stride < hq || d.q_seq_stride < 0 || d.q_out_seq_stride < 0 ||
+            (d.n_seqs > 1 && (d.q_seq_stride == 0 || d.q_out_seq_stride == 0)))
+            return bad("q / q_out strides");
+        if ((d.q_token_stride * is) % 16 || (d.q_seq_stride * is) % 16 || (d.q_out_token_stride * os) % 16 || (d.q_out_seq_stride * os) % 16)
+            return bad("q / q_out strides must be multiples of 16 bytes");
+        if (d.q == d.q_out && (d.in_dtype != d.q_out_dtype || d.q_token_stride != d.q_out_token_stride || d.q_seq_stride != d.q_out_seq_stride))
+            return bad("in-place queries need equal types and strides");
+    }
+    if (d.n_kv_heads == 0) return ok();
+    const int64_t hk = static_cast<int64_t>(d.n_kv_heads) * d.head_dim;
+    if (!d.k || !d.v || !aligned16(d.k) || !aligned16(d.v)) return bad("k / v null or not 16-byte aligned");
+    if (d.kv_token_stride < hk || d.kv_seq_stride < 0 || (d.n_seqs > 1 && d.kv_seq_stride == 0)) return bad("k / v strides");
+    if ((d.kv_token_stride * is) % 16 || (d.kv_seq_stride * is) % 16) return bad("k / v strides must be multiples of 16 bytes");
+    const int64_t rows = d.positions ? 0 : static_cast<int64_t>(d.start_position) + d.tokens;
+    if (d.cache_kind == ALPACA_CACHE_KV4) return validate_kv4_cache(d.kv4, d.n_seqs, d.n_kv_heads, d.head_dim, rows, "qkv");
+    if (d.cache_kind != ALPACA_CACHE_F32 && d.cache_kind != ALPACA_CACHE_F16) return bad("unknown cache kind");
+    const int64_t cs = d.cache_kind == ALPACA_CACHE_F16 ? 2 : 4;
+    if (!d.k_cache || !d.v_cache || !aligned16(d.k_cache) || !aligned16(d.v_cache)) return bad("caches null or not 16-byte aligned");
+    if (d.cache_row_stride < hk || d.cache_seq_stride < 0 || (d.n_seqs > 1 && d.cache_seq_stride == 0 && !d.block_table))
+        return bad("cache strides");
+    if ((d.cache_row_stride * cs) % 16 || (d.cache_seq_stride * cs) % 16) return bad("cache strides must be multiples of 16 bytes");
+    if (d.block_table) {
+        if (d.block_rows < 128 || d.block_rows % 128 || d.max_blocks < 1 || d.pool_blocks < 1 ||
+            d.block_stride < static_cast<int64_t>(d.block_rows) * d.cache_row_stride || (d.block_stride * cs) % 16)
+            return bad("a paged cache needs block_rows a multiple of 128, max_blocks and pool_blocks >= 1 and block_stride "
+                       "covering a block");
+        if (rows > static_cast<int64_t>(d.max_blocks) * d.block_rows) return bad("block table too short");
+    } else if (d.cache_rows < 1 || rows > d.cache_rows) {
+        return bad("rows past cache_rows");
+    }
+    return ok();
+}
+
+alpaca_cuda_status validate_kv4_read(const alpaca_kv4_read_desc* dp) {
+    if (!dp) return fail(ALPACA_CUDA_ERR_INVALID_ARGUMENT, "kv4_read: null descriptor");
+    const alpaca_kv4_read_desc& d = *dp;
+    auto bad = [&](const char* what) {
+        char sh[200];
+        std::snprintf(sh, sizeof(sh), "kv4_read: %s: seqs=%d rows=%d start=%d Hkv=%d d=%d", what, d.n_seqs, d.n_rows, d.start_row,
+                      d.n_kv_heads, d.head_dim);
+        return fail(ALPACA_CUDA_ERR_INVALID_ARGUMENT, sh);
+    };
+    if (d.n_seqs < 1 || d.n_seqs > 65535 || d.n_kv_heads < 1 || d.n_kv_heads > (1 << 20) || d.n_rows < 0 || d.start_row < 0) return bad("shapes");
+    if (!kv4_head_dim_ok(d.head_dim)) return bad("headDim must be a multiple of 32 up to 256");
+    if (!dtype_ok(d.out_dtype)) return bad("unknown dtype");
+    if (d.flags != 0) return bad("unknown flags");
+    if (d.start_row > (1 << 30) || d.n_rows > (1 << 30) - d.start_row) return bad("rows out of range");
+    if (!d.k_out || !d.v_out || !aligned16(d.k_out) || !aligned16(d.v_out)) return bad("outputs null or not 16-byte aligned");
+    const int64_t os = static_cast<int64_t>(dtype_size(d.out_dtype));
+    if (d.out_row_stride < static_cast<int64_t>(d.n_kv_heads) * d.head_dim || d.out_seq_stride < 0 ||
+        (d.n_seqs > 1 && d.out_seq_stride == 0) || (d.out_row_stride * os) % 16 || (d.out_seq_stride * os) % 16)
+        return bad("output strides must cover a row and be multiples of 16 bytes");
+    return validate_kv4_cache(d.cache, d.n_seqs, d.n_kv_heads, d.head_dim,
+                              d.row_starts ? 0 : static_cast<int64_t>(d.start_row) + d.n_rows, "kv4_read");
+}
+
+std::string kv4_shape(const alpaca_kv4_attn_desc& d) {
+    char sh[200];
+    std::snprintf(sh, sizeof(sh), "seqs=%d T=%d start=%d ctx<=%d H=%d/%d d=%d q=%s out=%s", d.n_seqs, d.tokens, d.start_position,
+                  d.max_ctx_len, d.n_heads, d.n_kv_heads, d.head_dim, d.q_dtype == ALPACA_F16 ? "f16" : "f32",
+                  d.out_dtype == ALPACA_F16 ? "f16" : "f32");
+    return sh;
+}
+
+alpaca_cuda_status validate_kv4_attn(const alpaca_kv4_attn_desc* dp) {
+    if (!dp) return fail(ALPACA_CUDA_ERR_INVALID_ARGUMENT, "kv4_attention: null descriptor");
+    const alpaca_kv4_attn_desc& d = *dp;
+    auto bad = [&](const char* what) {
+        return fail(ALPACA_CUDA_ERR_INVALID_ARGUMENT, std::string("kv4_attention: ") + what + ": " + kv4_shape(d));
+    };
+    if (d.n_seqs < 1 || d.n_seqs > 65535 || d.n_heads < 1 || d.n_kv_heads < 1 || d.tokens < 1 || d.start_position < 0 ||
+        d.n_heads > (1 << 20))
+        return bad("shapes");
+    if (d.n_heads % d.n_kv_heads != 0) return bad("heads not a multiple of kvHeads");
+    if (!kv4_head_dim_ok(d.head_dim)) return bad("headDim must be a multiple of 32 up to 256");
+    if (!dtype_ok(d.q_dtype) || !dtype_ok(d.out_dtype)) return bad("unknown dtype");
+    if (d.flags & ~ALPACA_ATTN_FLAG_VARLEN) return bad("unknown flags");
+    if (!(d.scale >= 0.f) || !std::isfinite(d.scale)) return bad("scale must be finite and >= 0");
+    if (d.start_position > (1 << 30) || d.tokens > (1 << 30) - d.start_position) return bad("positions out of range");
+    const bool varlen = (d.flags & ALPACA_ATTN_FLAG_VARLEN) != 0;
+    if (varlen) {
+        if (d.ctx_lens) return bad("ctx_lens and the ragged prefill flag together");
+        if (!d.q_offsets || !d.start_positions) return bad("ragged prefill needs q_offsets and start_positions");
+        if (d.total_tokens < 1 || d.max_ctx_len < 1) return bad("ragged prefill needs total_tokens >= 1 and max_ctx_len >= 1");
+        if (static_cast<int64_t>(d.n_seqs) * ((d.tokens + 255) / 256) > (1 << 26)) return bad("ragged prefill has too many sequences");
+    }
+    if ((varlen || d.ctx_lens) && (d.max_ctx_len < 0 || d.max_ctx_len > (1 << 30))) return bad("max_ctx_len out of range");
+    if (!d.q || !d.out || !aligned16(d.q) || !aligned16(d.out)) return bad("q / out null or not 16-byte aligned");
+    const int64_t hq = static_cast<int64_t>(d.n_heads) * d.head_dim;
+    const int64_t qs = static_cast<int64_t>(dtype_size(d.q_dtype)), os = static_cast<int64_t>(dtype_size(d.out_dtype));
+    if (d.q_token_stride < hq || d.out_token_stride < hq || d.q_seq_stride < 0 || d.out_seq_stride < 0 ||
+        (!varlen && d.n_seqs > 1 && (d.q_seq_stride == 0 || d.out_seq_stride == 0)))
+        return bad("q / out strides");
+    if ((d.q_token_stride * qs) % 16 || (d.q_seq_stride * qs) % 16 || (d.out_token_stride * os) % 16 || (d.out_seq_stride * os) % 16)
+        return bad("strides must be multiples of 16 bytes");
+    const int64_t rows = (d.ctx_lens || varlen) ? d.max_ctx_len : static_cast<int64_t>(d.start_position) + d.tokens;
+    return validate_kv4_cache(d.cache, d.n_seqs, d.n_kv_heads, d.head_dim, rows, "kv4_attention");
+}
+
+bool kv4_fast_head_dim(const alpaca_kv4_attn_desc& d) { return d.head_dim == 64 || d.head_dim == 128; }
+
+alpaca_attn_kernel kv4_select(const alpaca_kv4_attn_desc& d) {
+    if (d.flags & ALPACA_ATTN_FLAG_VARLEN) return ALPACA_ATTN_PREFILL_TC;
+    if (!kv4_fast_head_dim(d)) return ALPACA_ATTN_GENERAL;
+    return (d.tokens >= kPrefillMinTokens && !d.ctx_lens) ? ALPACA_ATTN_PREFILL_TC : ALPACA_ATTN_DECODE_SPLIT;
+}
+
+// Descriptor checks, then the kernel choice (ALPACA_ATTN_AUTO resolved) and its limits.
+alpaca_cuda_status kv4_prepare(const alpaca_kv4_attn_desc* dp, alpaca_attn_kernel& kind) {
+    const alpaca_cuda_status st = validate_kv4_attn(dp);
+    if (st != ALPACA_CUDA_OK) return st;
+    if (kind == ALPACA_ATTN_AUTO) kind = kv4_select(*dp);
+    const bool varlen = (dp->flags & ALPACA_ATTN_FLAG_VARLEN) != 0;
+    auto no = [&](const char* what) {
+        return fail(ALPACA_CUDA_ERR_UNSUPPORTED, std::string("kv4_attention: ") + what + ": " + kv4_shape(*dp));
+    };
+    if (varlen && kind != ALPACA_ATTN_PREFILL_TC) return no("the ragged prefill form is served by the tensor-core prefill only");
+    switch (kind) {
+        case ALPACA_ATTN_PREFILL_TC:
+            if (!kv4_fast_head_dim(*dp)) return no("tensor-core prefill needs headDim 64/128");
+            if (dp->ctx_lens) return no("tensor-core prefill takes start_position or the ragged form, not ctx_lens");
+            return ok();
+        case ALPACA_ATTN_DECODE_SPLIT:
+            if (!kv4_fast_head_dim(*dp)) return no("the split kernel needs headDim 64/128");
+            return ok();
+        case ALPACA_ATTN_GENERAL: return ok();
+        default: return fail(ALPACA_CUDA_ERR_INVALID_ARGUMENT, "kv4_attention: unknown kernel kind");
+    }
+}
+
 }  // namespace
 }  // namespace alpaca
 
@@ -478,6 +668,61 @@ alpaca_cuda_status alpaca_decode_project(const alpaca_proj_desc* dp, alpaca_stre
     const alpaca_cuda_status st = device_for(s, "project", &di);
     if (st != ALPACA_CUDA_OK) return st;
     return launched(launch_proj(d, di.num_sms, s), "project");
+}
+
+alpaca_cuda_status alpaca_qkv_append(const alpaca_qkv_desc* desc, alpaca_stream_t stream) {
+    alpaca_cuda_status st = validate_qkv(desc);
+    if (st != ALPACA_CUDA_OK) return st;
+    const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    DeviceInfo di;
+    st = device_for(s, "qkv", &di);
+    if (st != ALPACA_CUDA_OK) return st;
+    return launched(launch_qkv_append(*desc, di.err, s), "qkv");
+}
+
+alpaca_cuda_status alpaca_kv4_read(const alpaca_kv4_read_desc* desc, alpaca_stream_t stream) {
+    alpaca_cuda_status st = validate_kv4_read(desc);
+    if (st != ALPACA_CUDA_OK || desc->n_rows == 0) return st;
+    const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    DeviceInfo di;
+    st = device_for(s, "kv4_read", &di);
+    if (st != ALPACA_CUDA_OK) return st;
+    return launched(launch_kv4_read(*desc, nullptr, nullptr, di.err, s), "kv4_read");
+}
+
+alpaca_cuda_status alpaca_kv4_attention(const alpaca_kv4_attn_desc* desc, alpaca_attn_kernel kind, void* workspace,
+                                        size_t workspace_bytes, alpaca_stream_t stream) {
+    alpaca_cuda_status st = kv4_prepare(desc, kind);
+    if (st != ALPACA_CUDA_OK) return st;
+    const size_t need = kv4_workspace_bytes(*desc, kind);
+    if (need > 0 && (workspace_bytes < need || !workspace))
+        return fail(ALPACA_CUDA_ERR_WORKSPACE_TOO_SMALL, "kv4_attention: workspace of " + std::to_string(workspace_bytes) +
+                                                             " bytes, " + std::to_string(need) + " needed");
+    if (need > 0 && !aligned16(workspace))
+        return fail(ALPACA_CUDA_ERR_INVALID_ARGUMENT, "kv4_attention: workspace must be 16-byte aligned");
+    const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    DeviceInfo di;
+    st = device_for(s, "kv4_attention", &di);
+    if (st != ALPACA_CUDA_OK) return st;
+    const float scale = desc->scale > 0.f ? desc->scale : 1.0f / std::sqrt(static_cast<float>(desc->head_dim));
+    return launched(launch_kv4_attention(*desc, kind, scale, workspace, workspace_bytes, di.err, di.num_sms, s), "kv4_attention");
+}
+
+alpaca_cuda_status alpaca_kv4_workspace_bytes(const alpaca_kv4_attn_desc* desc, alpaca_attn_kernel kind, size_t* bytes) {
+    if (!bytes) return fail(ALPACA_CUDA_ERR_INVALID_ARGUMENT, "kv4_workspace_bytes: null output");
+    const alpaca_cuda_status st = kv4_prepare(desc, kind);
+    if (st != ALPACA_CUDA_OK) return st;
+    *bytes = kv4_workspace_bytes(*desc, kind);
+    return ok();
+}
+
+alpaca_cuda_status alpaca_kv4_select(const alpaca_kv4_attn_desc* desc, alpaca_attn_kernel* kind) {
+    if (!kind) return fail(ALPACA_CUDA_ERR_INVALID_ARGUMENT, "kv4_select: null output");
+    alpaca_attn_kernel k = ALPACA_ATTN_AUTO;
+    const alpaca_cuda_status st = kv4_prepare(desc, k);
+    if (st != ALPACA_CUDA_OK) return st;
+    *kind = k;
+    return ok();
 }
 
 alpaca_cuda_status alpaca_attention_workspace_bytes(const alpaca_attn_desc* desc, alpaca_attn_kernel kind,

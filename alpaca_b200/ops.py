@@ -16,12 +16,13 @@ theta:)`` (MetalOps.swift:165-171): a host f32 [tokens, heads, head_dim] array r
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import numpy as np
 import torch
 
-from ._lib import (FLAG_VARLEN, PROJ_ADD, PROJ_NORM, PROJ_SILU, AlpacaCUDAError, AttnDesc, DType, Kernel,
-                   ProjDesc, RopeDesc, Status, WeightFormat, check, load)
+from ._lib import (FLAG_VARLEN, PROJ_ADD, PROJ_NORM, PROJ_SILU, AlpacaCUDAError, AttnDesc, CacheKind, DType, Kernel,
+                   Kv4AttnDesc, Kv4CacheDesc, Kv4ReadDesc, ProjDesc, QkvDesc, RopeDesc, Status, WeightFormat, check, load)
 
 KV_PADDING_ROWS = 32  # KernelEncoder.kvPaddingRows (KernelEncoder.swift:73)
 
@@ -363,3 +364,275 @@ def decode_project(weights: list[torch.Tensor], fmt: str, k: int, x: torch.Tenso
     d = make_proj_desc(weights, fmt, k, x, outs, norm_weight=norm_weight, eps=eps, silu_gate=silu_gate, add=add)
     project_launch(d, stream)
     return d
+
+
+# ---------------------------------------------------------------------------------------------- 4-bit KV cache
+
+class Kv4Cache(NamedTuple):
+    """One layer's 4-bit KV cache (alpaca_kv4_cache): codes uint8 [units, kv_heads, rows, head_dim / 2] and scales int16
+    [units, kv_heads, rows, head_dim / 32] of K and V. A unit is one sequence's cache, or a block of a pool."""
+    k_codes: torch.Tensor
+    k_scales: torch.Tensor
+    v_codes: torch.Tensor
+    v_scales: torch.Tensor
+
+
+def kv4_cache(units: int, rows: int, kv_heads: int, head_dim: int, device: str | int | torch.device = "cuda") -> Kv4Cache:
+    """A zeroed 4-bit cache of `units` sequences (or pool blocks) of at least `rows` rows (rounded up to 16)."""
+    if units < 1 or rows < 1 or kv_heads < 1 or head_dim % 32 or not 32 <= head_dim <= 256:
+        raise AlpacaCUDAError(Status.INVALID_ARGUMENT, f"kv4_cache: {units} x {rows} rows, {kv_heads} heads of {head_dim}")
+    rows = (rows + 15) // 16 * 16
+    codes = [torch.zeros((units, kv_heads, rows, head_dim // 2), dtype=torch.uint8, device=device) for _ in range(2)]
+    scales = [torch.zeros((units, kv_heads, rows, head_dim // 32), dtype=torch.int16, device=device) for _ in range(2)]
+    return Kv4Cache(codes[0], scales[0], codes[1], scales[1])
+
+
+def _kv4_desc(cache: Kv4Cache, seqs: int, block_table: torch.Tensor | None) -> tuple[Kv4CacheDesc, int, int]:
+    """(descriptor, kv heads, head_dim) of a cache that `seqs` sequences use."""
+    kc, ks, vc, vs = cache
+    if kc.dim() != 4 or kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or kc.shape != vc.shape or kc.stride() != vc.stride():
+        raise AlpacaCUDAError(Status.INVALID_ARGUMENT, "kv4: codes must be uint8 [units, kv_heads, rows, head_dim / 2], K and V alike")
+    units, heads, rows, half = kc.shape
+    want = (units, heads, rows, half // 16)
+    if ks.dtype != torch.int16 or vs.dtype != torch.int16 or tuple(ks.shape) != want or tuple(vs.shape) != want or \
+            ks.stride() != vs.stride():
+        raise AlpacaCUDAError(Status.INVALID_ARGUMENT, "kv4: scales must be int16 [units, kv_heads, rows, head_dim / 32], K and V alike")
+    if kc.stride(-1) != 1 or kc.stride(-2) != half or ks.stride(-1) != 1 or ks.stride(-2) != half // 16:
+        raise AlpacaCUDAError(Status.INVALID_ARGUMENT, "kv4: a head's rows must be contiguous")
+    d = Kv4CacheDesc()
+    d.k_codes, d.v_codes, d.k_scales, d.v_scales = kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr()
+    d.code_head_stride, d.code_unit_stride = kc.stride(1), kc.stride(0) if units > 1 else 0
+    d.scale_head_stride, d.scale_unit_stride = ks.stride(1), ks.stride(0) if units > 1 else 0
+    d.rows = rows
+    if block_table is not None:
+        if block_table.dtype != torch.int32 or not block_table.is_cuda or block_table.dim() != 2 or \
+                block_table.shape[0] != seqs or not block_table.is_contiguous():
+            raise AlpacaCUDAError(Status.INVALID_ARGUMENT, "block_table must be a contiguous CUDA int32 [seqs, blocks]")
+        d.block_table, d.max_blocks, d.pool_blocks = block_table.data_ptr(), block_table.shape[1], units
+    elif units != seqs:
+        raise AlpacaCUDAError(Status.INVALID_ARGUMENT, f"kv4: {units} caches for {seqs} sequences")
+    return d, heads, half * 2
+
+
+def _i32_vector(t: torch.Tensor, n: int, name: str) -> int:
+    if t.dtype != torch.int32 or not t.is_cuda or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+        raise AlpacaCUDAError(Status.INVALID_ARGUMENT, f"{name} must be a contiguous CUDA int32 [{n}]")
+    return t.data_ptr()
+
+
+def make_qkv_desc(q: torch.Tensor | None, k: torch.Tensor | None, v: torch.Tensor | None, q_out: torch.Tensor | None,
+                  cache: "Kv4Cache | tuple[torch.Tensor, torch.Tensor] | None", *, theta: float, start_position: int = 0,
+                  positions: torch.Tensor | None = None, interleaved: bool = True, q_norm: torch.Tensor | None = None,
+                  k_norm: torch.Tensor | None = None, eps: float = 1e-5, block_table: torch.Tensor | None = None) -> QkvDesc:
+    """Descriptor of alpaca_qkv_append: q [S,T,H,d] -> q_out [S,T,H,d] (may be q), k / v [S,T,Hkv,d] -> `cache`, a Kv4Cache
+    or a (k_cache, v_cache) pair of f16 / f32 rows [S,rows,Hkv,d]; with `block_table` (CUDA int32 [S, max_blocks]) the cache
+    is a block pool. q_norm / k_norm: f32 [d] RMSNorm weights of the query / key heads. (q, q_out) or (k, v, cache) may be
+    None. 3-D tensors mean S = 1."""
+    d_ = QkvDesc()
+    ref = q if q is not None else k
+    if ref is None:
+        raise AlpacaCUDAError(Status.INVALID_ARGUMENT, "qkv: neither q nor k given")
+    r4 = _as4(ref, "q" if q is not None else "k")
+    S, T, _, D = r4.shape
+    d_.n_seqs, d_.tokens, d_.head_dim, d_.start_position = S, T, D, int(start_position)
+    if positions is not None:
+        d_.positions = _i32_vector(positions, S, "positions")
+    d_.theta, d_.eps, d_.interleaved, d_.in_dtype = float(theta), float(eps), 1 if interleaved else 0, _dtype(r4)
+    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if w is not None:
+            if w.dtype != torch.float32 or not w.is_cuda or w.shape != (D,) or not w.is_contiguous():
+                raise AlpacaCUDAError(Status.INVALID_ARGUMENT, f"qkv: {name} must be a contiguous CUDA f32 [head_dim]")
+            setattr(d_, name, w.data_ptr())
+    if q is not None:
+        if q_out is None:
+            raise AlpacaCUDAError(Status.INVALID_ARGUMENT, "qkv: q without q_out")
+        o4 = _as4(q_out, "q_out")
+        if o4.shape != r4.shape:
+            raise AlpacaCUDAError(Status.INVALID_ARGUMENT, "qkv: q_out must have q's shape")
+        d_.n_heads, d_.q_out_dtype = r4.shape[2], _dtype(o4)
+        d_.q, d_.q_token_stride, d_.q_seq_stride = r4.data_ptr(), r4.stride(1), r4.stride(0) if S > 1 else 0
+        d_.q_out, d_.q_out_token_stride, d_.q_out_seq_stride = o4.data_ptr(), o4.stride(1), o4.stride(0) if S > 1 else 0
+    if k is not None:
+        if v is None or cache is None:
+            raise AlpacaCUDAError(Status.INVALID_ARGUMENT, "qkv: k without v and a cache")
+        k4, v4 = _as4(k, "k"), _as4(v, "v")
+        if k4.dtype != r4.dtype or v4.dtype != r4.dtype or k4.shape != v4.shape or k4.stride() != v4.stride() or \
+                k4.shape[:2] != (S, T) or k4.shape[3] != D:
+            raise AlpacaCUDAError(Status.INVALID_ARGUMENT, "qkv: q, k and v must share type, sequences, tokens and head_dim; "
+                                                           "k and v their strides")
+        d_.n_kv_heads = k4.shape[2]
+        d_.k, d_.v, d_.kv_token_stride, d_.kv_seq_stride = k4.data_ptr(), v4.data_ptr(), k4.stride(1), k4.stride(0) if S > 1 else 0
+        if isinstance(cache, Kv4Cache):
+            d_.cache_kind = CacheKind.KV4
+            d_.kv4, heads, dim = _kv4_desc(cache, S, block_table)
+            if (heads, dim) != (d_.n_kv_heads, D):
+                raise AlpacaCUDAError(Status.INVALID_ARGUMENT, f"qkv: cache of {heads} heads of {dim}")
+        else:
+            kc, vc = _as4(cache[0], "k_cache"), _as4(cache[1], "v_cache")
+            if kc.stride() != vc.stride() or kc.shape != vc.shape or kc.dtype != vc.dtype or kc.shape[2:] != k4.shape[2:]:
+                raise AlpacaCUDAError(Status.INVALID_ARGUMENT, "qkv: caches must share type and strides and hold k's heads")
+            d_.cache_kind = CacheKind.F16 if _dtype(kc) == DType.F16 else CacheKind.F32
+            d_.k_cache, d_.v_cache, d_.cache_row_stride = kc.data_ptr(), vc.data_ptr(), kc.stride(1)
+            if block_table is not None:
+                if block_table.dtype != torch.int32 or not block_table.is_cuda or block_table.dim() != 2 or \
+                        block_table.shape[0] != S or not block_table.is_contiguous():
+                    raise AlpacaCUDAError(Status.INVALID_ARGUMENT, "block_table must be a contiguous CUDA int32 [seqs, blocks]")
+                d_.block_table, d_.max_blocks = block_table.data_ptr(), block_table.shape[1]
+                d_.block_rows, d_.pool_blocks, d_.block_stride = kc.shape[1], kc.shape[0], kc.stride(0)
+            else:
+                if kc.shape[0] != S:
+                    raise AlpacaCUDAError(Status.INVALID_ARGUMENT, f"qkv: {kc.shape[0]} caches for {S} sequences")
+                d_.cache_rows, d_.cache_seq_stride = kc.shape[1], kc.stride(0) if S > 1 else 0
+    return d_
+
+
+def qkv_launch(desc: QkvDesc, stream: torch.cuda.Stream | None = None) -> None:
+    s = stream if stream is not None else torch.cuda.current_stream()
+    check(load().alpaca_qkv_append(ctypes.byref(desc), s.cuda_stream))
+
+
+def qkv_append(q: torch.Tensor | None, k: torch.Tensor | None, v: torch.Tensor | None, q_out: torch.Tensor | None,
+               cache: "Kv4Cache | tuple[torch.Tensor, torch.Tensor] | None", *, theta: float, start_position: int = 0,
+               positions: torch.Tensor | None = None, interleaved: bool = True, q_norm: torch.Tensor | None = None,
+               k_norm: torch.Tensor | None = None, eps: float = 1e-5, block_table: torch.Tensor | None = None,
+               stream: torch.cuda.Stream | None = None) -> QkvDesc:
+    """Enqueue head norms + RoPE + KV append in one pass (make_qkv_desc)."""
+    d_ = make_qkv_desc(q, k, v, q_out, cache, theta=theta, start_position=start_position, positions=positions,
+                       interleaved=interleaved, q_norm=q_norm, k_norm=k_norm, eps=eps, block_table=block_table)
+    qkv_launch(d_, stream)
+    return d_
+
+
+def make_kv4_read_desc(cache: Kv4Cache, k_out: torch.Tensor, v_out: torch.Tensor, *, start_row: int = 0,
+                       row_starts: torch.Tensor | None = None, block_table: torch.Tensor | None = None) -> Kv4ReadDesc:
+    """Descriptor of alpaca_kv4_read: rows start .. start + T - 1 of every sequence into k_out / v_out [S,T,Hkv,d] (f16 or
+    f32), start = row_starts[s] (CUDA int32 [S]) or start_row."""
+    k4, v4 = _as4(k_out, "k_out"), _as4(v_out, "v_out")
+    if k4.shape != v4.shape or k4.stride() != v4.stride() or k4.dtype != v4.dtype:
+        raise AlpacaCUDAError(Status.INVALID_ARGUMENT, "kv4_read: k_out and v_out must share shape, type and strides")
+    S, T, H, D = k4.shape
+    d_ = Kv4ReadDesc()
+    d_.n_seqs, d_.n_rows, d_.n_kv_heads, d_.head_dim, d_.start_row = S, T, H, D, int(start_row)
+    d_.out_dtype = _dtype(k4)
+    if row_starts is not None:
+        d_.row_starts = _i32_vector(row_starts, S, "row_starts")
+    d_.cache, heads, dim = _kv4_desc(cache, S, block_table)
+    if (heads, dim) != (H, D):
+        raise AlpacaCUDAError(Status.INVALID_ARGUMENT, f"kv4_read: cache of {heads} heads of {dim}, outputs of {H} of {D}")
+    d_.k_out, d_.v_out, d_.out_row_stride = k4.data_ptr(), v4.data_ptr(), k4.stride(1)
+    d_.out_seq_stride = k4.stride(0) if S > 1 else 0
+    return d_
+
+
+def kv4_read_launch(desc: Kv4ReadDesc, stream: torch.cuda.Stream | None = None) -> None:
+    s = stream if stream is not None else torch.cuda.current_stream()
+    check(load().alpaca_kv4_read(ctypes.byref(desc), s.cuda_stream))
+
+
+def kv4_read(cache: Kv4Cache, k_out: torch.Tensor, v_out: torch.Tensor, *, start_row: int = 0,
+             row_starts: torch.Tensor | None = None, block_table: torch.Tensor | None = None,
+             stream: torch.cuda.Stream | None = None) -> Kv4ReadDesc:
+    """Enqueue the read-back of 4-bit cache rows as values (make_kv4_read_desc)."""
+    d_ = make_kv4_read_desc(cache, k_out, v_out, start_row=start_row, row_starts=row_starts, block_table=block_table)
+    kv4_read_launch(d_, stream)
+    return d_
+
+
+def make_kv4_attn_desc(q: torch.Tensor, cache: Kv4Cache, out: torch.Tensor, *, start_position: int = 0,
+                       ctx_lens: torch.Tensor | None = None, max_ctx_len: int | None = None, scale: float = 0.0,
+                       block_table: torch.Tensor | None = None) -> Kv4AttnDesc:
+    """Descriptor of alpaca_kv4_attention for q, out [S,T,H,d] over the sequences' 4-bit caches. The call's last token sits on
+    row ctx - 1 of its sequence, ctx = ctx_lens[s] (CUDA int32 [S], entries 0 .. max_ctx_len) or start_position + T."""
+    q4, o4 = _as4(q, "q"), _as4(out, "out")
+    if q4.shape != o4.shape:
+        raise AlpacaCUDAError(Status.INVALID_ARGUMENT, "kv4_attention: out must have q's shape")
+    S, T, H, D = q4.shape
+    d_ = Kv4AttnDesc()
+    d_.n_seqs, d_.tokens, d_.n_heads, d_.head_dim, d_.start_position = S, T, H, D, int(start_position)
+    d_.cache, d_.n_kv_heads, dim = _kv4_desc(cache, S, block_table)
+    if dim != D:
+        raise AlpacaCUDAError(Status.INVALID_ARGUMENT, f"kv4_attention: queries of {D} channels over a cache of {dim}")
+    if ctx_lens is not None:
+        d_.ctx_lens = _i32_vector(ctx_lens, S, "ctx_lens")
+        room = d_.cache.rows * (d_.cache.max_blocks if block_table is not None else 1)
+        d_.max_ctx_len = int(max_ctx_len if max_ctx_len is not None else room)
+    d_.q_dtype, d_.out_dtype = _dtype(q4), _dtype(o4)
+    d_.q, d_.q_token_stride, d_.q_seq_stride = q4.data_ptr(), q4.stride(1), q4.stride(0) if S > 1 else 0
+    d_.out, d_.out_token_stride, d_.out_seq_stride = o4.data_ptr(), o4.stride(1), o4.stride(0) if S > 1 else 0
+    d_.scale = float(scale)
+    return d_
+
+
+def make_kv4_varlen_desc(q: torch.Tensor, cache: Kv4Cache, out: torch.Tensor, q_offsets: torch.Tensor,
+                         start_positions: torch.Tensor, *, max_tokens: int, max_ctx_len: int, scale: float = 0.0,
+                         block_table: torch.Tensor | None = None) -> Kv4AttnDesc:
+    """Descriptor of a ragged prefill over 4-bit caches: q, out packed [total_tokens, H, d], the rest as make_varlen_desc."""
+    S = start_positions.numel()
+    if q.dim() != 3 or out.shape != q.shape:
+        raise AlpacaCUDAError(Status.INVALID_ARGUMENT, "ragged q and out must be packed [total_tokens, heads, head_dim]")
+    q4, o4 = _as4(q, "q"), _as4(out, "out")
+    d_ = Kv4AttnDesc()
+    d_.n_seqs, d_.tokens, d_.n_heads, d_.head_dim = S, int(max_tokens), q4.shape[2], q4.shape[3]
+    d_.cache, d_.n_kv_heads, dim = _kv4_desc(cache, S, block_table)
+    if dim != d_.head_dim:
+        raise AlpacaCUDAError(Status.INVALID_ARGUMENT, f"kv4_attention: queries of {d_.head_dim} channels over a cache of {dim}")
+    d_.flags, d_.max_ctx_len, d_.total_tokens = FLAG_VARLEN, int(max_ctx_len), q4.shape[1]
+    d_.q_offsets = _i32_vector(q_offsets, S + 1, "q_offsets")
+    d_.start_positions = _i32_vector(start_positions, S, "start_positions")
+    d_.q_dtype, d_.out_dtype = _dtype(q4), _dtype(o4)
+    d_.q, d_.q_token_stride, d_.out, d_.out_token_stride = q4.data_ptr(), q4.stride(1), o4.data_ptr(), o4.stride(1)
+    d_.scale = float(scale)
+    return d_
+
+
+def kv4_workspace_bytes(desc: Kv4AttnDesc, kind: Kernel = Kernel.AUTO) -> int:
+    n = ctypes.c_size_t(0)
+    check(load().alpaca_kv4_workspace_bytes(ctypes.byref(desc), int(kind), ctypes.byref(n)))
+    return int(n.value)
+
+
+def kv4_select(desc: Kv4AttnDesc) -> Kernel:
+    k = ctypes.c_int(0)
+    check(load().alpaca_kv4_select(ctypes.byref(desc), ctypes.byref(k)))
+    return Kernel(k.value)
+
+
+def kv4_attention_launch(desc: Kv4AttnDesc, workspace: torch.Tensor | None = None, kind: Kernel = Kernel.AUTO,
+                         stream: torch.cuda.Stream | None = None) -> None:
+    """Enqueue one call of alpaca_kv4_attention on `stream` (default: torch's current stream)."""
+    s = stream if stream is not None else torch.cuda.current_stream()
+    ws_ptr = workspace.data_ptr() if workspace is not None else None
+    ws_len = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    check(load().alpaca_kv4_attention(ctypes.byref(desc), int(kind), ws_ptr, ws_len, s.cuda_stream))
+
+
+def kv4_attention(q: torch.Tensor, cache: Kv4Cache, out: torch.Tensor, *, start_position: int = 0,
+                  ctx_lens: torch.Tensor | None = None, max_ctx_len: int | None = None, scale: float = 0.0,
+                  block_table: torch.Tensor | None = None, kind: Kernel = Kernel.AUTO, workspace: torch.Tensor | None = None,
+                  stream: torch.cuda.Stream | None = None) -> Kv4AttnDesc:
+    """Enqueue attention over the 4-bit cache (make_kv4_attn_desc); allocates the workspace with torch when none is given
+    or the one given is smaller than the library asks for (callers on a hot loop pass their own)."""
+    desc = make_kv4_attn_desc(q, cache, out, start_position=start_position, ctx_lens=ctx_lens, max_ctx_len=max_ctx_len,
+                              scale=scale, block_table=block_table)
+    _kv4_run(desc, kind, workspace, q.device, stream)
+    return desc
+
+
+def kv4_prefill_varlen(q: torch.Tensor, cache: Kv4Cache, out: torch.Tensor, q_offsets: torch.Tensor,
+                       start_positions: torch.Tensor, *, max_tokens: int, max_ctx_len: int, scale: float = 0.0,
+                       block_table: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+                       stream: torch.cuda.Stream | None = None) -> Kv4AttnDesc:
+    """Enqueue a ragged prefill over 4-bit caches (make_kv4_varlen_desc); workspace as for kv4_attention."""
+    desc = make_kv4_varlen_desc(q, cache, out, q_offsets, start_positions, max_tokens=max_tokens, max_ctx_len=max_ctx_len,
+                                scale=scale, block_table=block_table)
+    _kv4_run(desc, Kernel.AUTO, workspace, q.device, stream)
+    return desc
+
+
+def _kv4_run(desc: Kv4AttnDesc, kind: Kernel, workspace: torch.Tensor | None, device, stream) -> None:
+    need = kv4_workspace_bytes(desc, kind)
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        # allocated on the stream that uses it, so that its memory is not handed out again before the call has run
+        with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(device)):
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    kv4_attention_launch(desc, workspace, kind, stream)

@@ -303,6 +303,162 @@ typedef struct alpaca_proj_desc {
  * weight read once per pass of up to 4 rows (larger batches belong to a GEMM). */
 alpaca_cuda_status alpaca_decode_project(const alpaca_proj_desc* desc, alpaca_stream_t stream);
 
+/* ---- 4-bit KV cache: rows written with head norms and RoPE, read back, and attended over. alpaca.swift has no quantised
+ * cache and no q / k norms (its caches are KVPrecision.float16 / .float32, KernelEncoder.swift:9-17); these entry points
+ * extend its cache contract. */
+
+/* The 4-bit cache of one layer: 4.5 bits per value. A head row of head_dim channels is head_dim / 32 blocks of 32 channels.
+ *   scales  uint16 per block: the f16 bits of the block's step with the low 4 mantissa bits replaced by its zero point
+ *   codes   4 bits per channel, eight to a 32-bit little-endian word: channel 32 b + 8 t + n is nibble n of word
+ *           t * (head_dim / 32) + b of the row (t = 0..3)
+ *   value = (code - zero) * step
+ * Every value is exact in f16 (4 + 7 significant bits). Rows are quantised with the block's range widened to hold 0:
+ * lo = min(0, x..), hi = max(0, x..), step = the smallest f16 with 7 significant bits >= min((hi - lo) / 15, 4352),
+ * zero = clamp(round(-lo / step), 0, 15), code = clamp(round(x / step) + zero, 0, 15), in f32, ties to even: no value is
+ * off by more than half a step unless its block spans more than 65280. A block with a NaN or an infinity reads back as NaN.
+ * Layout: units of `rows` rows, [unit][n_kv_heads][rows], each head's rows contiguous (head_dim / 2 code bytes and
+ * head_dim / 32 scales per row), so that a head's rows stream as one run. A unit is a sequence's cache (block_table NULL),
+ * or a block of a pool: row r of sequence s is row r % rows of unit block_table[s * max_blocks + r / rows]. K and V share
+ * the layout. Pointers 16-byte aligned, strides multiples of 16 bytes, `rows` a multiple of 16. */
+typedef struct alpaca_kv4_cache {
+    void* k_codes;
+    void* v_codes;
+    void* k_scales;
+    void* v_scales;
+    int64_t code_head_stride;   /* bytes between heads of a unit, >= rows * head_dim / 2 */
+    int64_t code_unit_stride;   /* bytes between units */
+    int64_t scale_head_stride;  /* uint16 elements between heads of a unit, >= rows * head_dim / 32 */
+    int64_t scale_unit_stride;  /* uint16 elements between units */
+    int32_t rows;               /* rows of a unit, a multiple of 16 */
+    int32_t max_blocks;         /* paged: entries of a sequence's table row */
+    const int32_t* block_table; /* paged: DEVICE [n_seqs][max_blocks], entries in [0, pool_blocks); NULL: contiguous */
+    int32_t pool_blocks;        /* paged: units of the pool */
+    int32_t reserved0;
+} alpaca_kv4_cache;
+
+/* Which cache alpaca_qkv_append writes: rows of values (the layouts of alpaca_rope_desc), or the 4-bit cache. */
+typedef enum alpaca_cache_kind {
+    ALPACA_CACHE_F32 = 0,
+    ALPACA_CACHE_F16 = 1,
+    ALPACA_CACHE_KV4 = 2
+} alpaca_cache_kind;
+
+/* One pass over the new tokens' projections: every query and key head is RMS-normalised over head_dim (where its norm
+ * weight is given: x * (1 / sqrt(mean(x^2) + eps)) * w, f32), queries and keys are rotated as alpaca_rope_kv_append
+ * rotates them (without norms the results equal that call's bit for bit), queries go to q_out, and rotated keys and raw
+ * values to the cache rows of their positions: token t of sequence s at (positions ? positions[s] : start_position) + t.
+ * A position outside the cache, or a table entry outside the pool, writes no cache row and is reported by
+ * alpaca_cuda_device_status; its queries are still written.
+ * q_out may be q itself (same type and strides). Pointers 16-byte aligned, strides in elements and multiples of 16 bytes. */
+typedef struct alpaca_qkv_desc {
+    int32_t n_seqs;           /* 1 .. 65535 */
+    int32_t n_heads;          /* query heads (0: no queries) */
+    int32_t n_kv_heads;       /* KV heads (0: no append) */
+    int32_t head_dim;         /* multiple of 32, 32 .. 256 */
+    int32_t tokens;           /* new tokens per sequence, >= 1 */
+    int32_t start_position;   /* position of token 0 when positions is NULL, >= 0 */
+    const int32_t* positions; /* optional DEVICE [n_seqs] */
+    float theta;              /* RoPE base, > 0 */
+    float eps;                /* of the norms, > 0 where one is given */
+    int32_t interleaved;      /* pair convention, as in alpaca_rope_desc */
+    int32_t in_dtype;         /* alpaca_dtype of q, k and v */
+    int32_t q_out_dtype;      /* alpaca_dtype of q_out */
+    int32_t cache_kind;       /* alpaca_cache_kind */
+    const float* q_norm;      /* DEVICE [head_dim], or NULL */
+    const float* k_norm;      /* DEVICE [head_dim], or NULL */
+    const void* q;            /* [n_seqs][tokens][n_heads][head_dim] */
+    int64_t q_token_stride;
+    int64_t q_seq_stride;
+    void* q_out;
+    int64_t q_out_token_stride;
+    int64_t q_out_seq_stride;
+    const void* k;            /* [n_seqs][tokens][n_kv_heads][head_dim] */
+    const void* v;
+    int64_t kv_token_stride;
+    int64_t kv_seq_stride;
+    /* ALPACA_CACHE_F32 / _F16: rows [n_kv_heads][head_dim], contiguous caches or pools as in alpaca_rope_desc */
+    void* k_cache;
+    void* v_cache;
+    int64_t cache_row_stride;
+    int64_t cache_seq_stride;
+    const int32_t* block_table;
+    int64_t block_stride;
+    int32_t block_rows;       /* a multiple of 128 */
+    int32_t max_blocks;
+    int32_t pool_blocks;
+    int32_t cache_rows;       /* rows of each contiguous cache, >= 1 */
+    alpaca_kv4_cache kv4;     /* ALPACA_CACHE_KV4 */
+    uint32_t flags;           /* 0 */
+    uint32_t reserved0;
+} alpaca_qkv_desc;
+
+/* Enqueue the pass on `stream`. */
+alpaca_cuda_status alpaca_qkv_append(const alpaca_qkv_desc* desc, alpaca_stream_t stream);
+
+/* Rows [start, start + n_rows) of every sequence's 4-bit cache (start = row_starts ? row_starts[s] : start_row) as values,
+ * in the layout of the f16 cache: [n_seqs][n_rows][n_kv_heads][head_dim], f16 (exact) or f32. Rows outside the cache or the
+ * pool read as zero and are reported by alpaca_cuda_device_status. */
+typedef struct alpaca_kv4_read_desc {
+    int32_t n_seqs;            /* 1 .. 65535 */
+    int32_t n_kv_heads;        /* >= 1 */
+    int32_t head_dim;          /* multiple of 32, 32 .. 256 */
+    int32_t n_rows;            /* >= 0; 0 enqueues nothing */
+    int32_t start_row;         /* >= 0 */
+    int32_t out_dtype;         /* alpaca_dtype */
+    const int32_t* row_starts; /* optional DEVICE [n_seqs] */
+    alpaca_kv4_cache cache;
+    void* k_out;
+    void* v_out;
+    int64_t out_row_stride;    /* elements, >= n_kv_heads * head_dim */
+    int64_t out_seq_stride;
+    uint32_t flags;            /* 0 */
+    uint32_t reserved0;
+} alpaca_kv4_read_desc;
+
+alpaca_cuda_status alpaca_kv4_read(const alpaca_kv4_read_desc* desc, alpaca_stream_t stream);
+
+/* Causal grouped-query attention over the 4-bit cache. The last of `tokens` query tokens of sequence s sits on row
+ * ctx - 1 of its cache, ctx = ctx_lens ? ctx_lens[s] : start_position + tokens: token t sees rows 0 .. ctx - tokens + t.
+ * ctx_lens entries lie in [0, max_ctx_len]; a token that sees no row (an empty context, or ctx < tokens) gives zeros.
+ * With ALPACA_ATTN_FLAG_VARLEN the call is a ragged prefill: q_offsets, start_positions, total_tokens, tokens and
+ * max_ctx_len as in alpaca_attn_desc.
+ * Kernels (alpaca_attn_kernel): DECODE_SPLIT (head_dim 64 / 128, any token count: a few tokens over long contexts; f32
+ * accuracy), PREFILL_TC (head_dim 64 / 128, uniform start_position or VARLEN: the visible rows are decoded to f16 in the
+ * workspace, exactly, and the tensor-core prefill runs over them with its accuracy, P rounded to f16), GENERAL (any
+ * head_dim). AUTO: PREFILL_TC for VARLEN and for 8 or more tokens at a uniform position, else DECODE_SPLIT, else GENERAL
+ * for other head dims. */
+typedef struct alpaca_kv4_attn_desc {
+    int32_t n_seqs;          /* 1 .. 65535 */
+    int32_t n_heads;
+    int32_t n_kv_heads;      /* n_heads % n_kv_heads == 0 */
+    int32_t head_dim;        /* multiple of 32, 32 .. 256 */
+    int32_t tokens;          /* >= 1 */
+    int32_t start_position;  /* >= 0, when ctx_lens is NULL */
+    const int32_t* ctx_lens; /* optional DEVICE [n_seqs] */
+    int32_t max_ctx_len;     /* bound of the contexts, with ctx_lens (>= 0) or VARLEN (>= 1) */
+    int32_t q_dtype;
+    int32_t out_dtype;
+    uint32_t flags;          /* ALPACA_ATTN_FLAG_NONE or ALPACA_ATTN_FLAG_VARLEN */
+    const void* q;           /* [n_seqs][tokens][n_heads][head_dim] */
+    int64_t q_token_stride;
+    int64_t q_seq_stride;
+    void* out;               /* [n_seqs][tokens][n_heads][head_dim] */
+    int64_t out_token_stride;
+    int64_t out_seq_stride;
+    float scale;             /* 0 selects 1 / sqrt(head_dim) */
+    int32_t total_tokens;    /* VARLEN */
+    const int32_t* q_offsets;
+    const int32_t* start_positions;
+    alpaca_kv4_cache cache;
+} alpaca_kv4_attn_desc;
+
+/* Enqueue the attention on `stream`; the workspace is at least alpaca_kv4_workspace_bytes, 16-byte aligned. */
+alpaca_cuda_status alpaca_kv4_attention(const alpaca_kv4_attn_desc* desc, alpaca_attn_kernel kind, void* workspace,
+                                        size_t workspace_bytes, alpaca_stream_t stream);
+alpaca_cuda_status alpaca_kv4_workspace_bytes(const alpaca_kv4_attn_desc* desc, alpaca_attn_kernel kind, size_t* bytes);
+/* Which kernel ALPACA_ATTN_AUTO would run (host-only). */
+alpaca_cuda_status alpaca_kv4_select(const alpaca_kv4_attn_desc* desc, alpaca_attn_kernel* kind);
+
 /* Synchronises `stream`, then reports and (when `clear` != 0) resets the device-side error word of that stream on the
  * current device: ALPACA_CUDA_ERR_DEVICE_TIMEOUT when a bounded wait gave up, ALPACA_CUDA_ERR_INVALID_ARGUMENT when
  * a device-side contract check failed (a block-table entry outside the pool, a ctx_lens entry outside
