@@ -482,6 +482,7 @@ alpaca_cuda_status validate_kv4_attn(const alpaca_kv4_attn_desc* dp) {
         d.n_heads > (1 << 20))
         return bad("shapes");
     if (d.n_heads % d.n_kv_heads != 0) return bad("heads not a multiple of kvHeads");
+    if (static_cast<int64_t>(d.n_seqs) * d.n_heads > (1 << 30) / d.tokens) return bad("too many query rows");
     if (!kv4_head_dim_ok(d.head_dim)) return bad("headDim must be a multiple of 32 up to 256");
     if (!dtype_ok(d.q_dtype) || !dtype_ok(d.out_dtype)) return bad("unknown dtype");
     if (d.flags & ~ALPACA_ATTN_FLAG_VARLEN) return bad("unknown flags");

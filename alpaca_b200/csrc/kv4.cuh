@@ -110,23 +110,44 @@ __device__ __forceinline__ uint4 kv4_word_values(uint32_t w, uint32_t header) {
                       __byte_perm(p26, p37, 0x7632));
 }
 
-// Header of a block with extremes lo <= 0 <= hi (NaN when the block held one): the smallest step of 7 significant bits
-// that is >= (hi - lo) / 15, and the zero point. Every finite value is then within half a step of a code, up to the
-// saturation of the step at kKv4MaxStep.
-__device__ __forceinline__ uint32_t kv4_header(float lo, float hi, float& step, float& zero) {
-    if (!(hi <= FLT_MAX && lo >= -FLT_MAX)) {
-        step = zero = 0.f;
-        return kKv4NanHeader;
-    }
-    const float s = fminf((hi - lo) / 15.f, kKv4MaxStep);
-    const uint32_t bits = (static_cast<uint32_t>(__half_as_ushort(__float2half_ru(s))) + 15u) & kKv4StepMask;
-    step = __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
-    zero = step > 0.f ? fminf(fmaxf(rintf(-lo / step), 0.f), 15.f) : 0.f;
-    return bits | static_cast<uint32_t>(zero);
+// A block's quantiser.
+struct Kv4Block {
+    uint32_t header;
+    float step, inv;  // inv = 1 / step, correctly rounded; both 0 where every code is 0
+    int bias;         // zero point less the bits of 1.5 * 2^23
+    bool wide;        // the step is saturated: values may lie beyond the codes
+};
+
+// From the block's extremes lo <= 0 <= hi (NaN when it held one): the smallest step of 7 significant bits that is
+// >= (hi - lo) / 15, and the zero point. Every finite value is then within half a step of a code, up to the saturation of
+// the step at kKv4MaxStep.
+__device__ __forceinline__ Kv4Block kv4_block(float lo, float hi) {
+    Kv4Block b;
+    b.step = b.inv = 0.f;
+    b.bias = 0;
+    b.wide = false;
+    b.header = kKv4NanHeader;
+    if (!(hi <= FLT_MAX && lo >= -FLT_MAX)) return b;
+    const float s = (hi - lo) / 15.f;
+    b.wide = s >= kKv4MaxStep;
+    const uint32_t bits = (static_cast<uint32_t>(__half_as_ushort(__float2half_ru(fminf(s, kKv4MaxStep)))) + 15u) & kKv4StepMask;
+    b.header = bits;
+    if (bits == 0) return b;
+    b.step = __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+    b.inv = 1.f / b.step;
+    const int zero = min(static_cast<int>(rintf(-lo / b.step)), 15);
+    b.header = bits | static_cast<uint32_t>(zero);
+    b.bias = zero - 0x4B400000;
+    return b;
 }
 
-__device__ __forceinline__ uint32_t kv4_code(float x, float step, float zero) {
-    return step > 0.f ? static_cast<uint32_t>(fminf(fmaxf(rintf(x / step) + zero, 0.f), 15.f)) : 0u;
+// clamp(round(x / step) + zero, 0, 15), the quotient as f32 division rounds it: from the correctly rounded reciprocal, one
+// residual step gives the correctly rounded quotient (Markstein, "Computation of elementary functions on the IBM RISC
+// System/6000 processor", 1990). Adding 1.5 * 2^23 rounds to an integer, ties to even, and leaves it in the low bits.
+__device__ __forceinline__ uint32_t kv4_code(float x, const Kv4Block& b) {
+    const float q = __fmul_rn(x, b.inv);
+    const float quotient = __fmaf_rn(__fmaf_rn(-q, b.step, x), b.inv, q);
+    return static_cast<uint32_t>(__vimin_s32_relu(__float_as_int(__fadd_rn(quotient, 12582912.f)) + b.bias, 15));
 }
 
 }  // namespace alpaca

@@ -11,8 +11,7 @@
 //   write      f16 / f32 row, or the blocks' steps, zero points and codes (kv4.cuh)
 // A row moves 4 d or 2 d bytes in and 0.56 d .. 4 d out: HBM for prompts, latency for one token per sequence.
 //
-// kv4_read_kernel: eight values of a row per thread and step, f16 or f32 out in the [seq][row][head][d] layout of the
-// f16 cache. It moves 0.56 d + 2 d (f16) bytes per row: HBM-bound.
+// kv4_read_kernel: four lanes per head row, f16 or f32 out in the [seq][row][head][d] layout of the f16 cache. It moves 0.56 d + 2 d (f16) bytes per row: HBM-bound.
 #include <cmath>
 
 #include "kv4.cuh"
@@ -32,7 +31,7 @@ struct AppendArgs {
     int64_t q_token_stride, q_seq_stride, kv_token_stride, kv_seq_stride, out_token_stride, out_seq_stride;
     const float* q_norm;
     const float* k_norm;
-    float eps;
+    float eps, inv_d;  // inv_d = 1 / d
     int in_f16, out_f16, interleaved;
     const int* positions;
     int start, n_heads, n_kv_heads, d, tokens, tpc;
@@ -88,89 +87,103 @@ __device__ __forceinline__ void store8(void* p, int64_t off, int f16, const floa
     }
 }
 
-// Row `row` of the CTA's tokens: its token, kind and head.
+// Rows of a CTA's tokens in order: row `i` (query heads, key heads, value heads) of its token `tt`. Lane groups step through
+// them by the CTA's rows per pass, without a division per row.
 struct RowAt {
-    int tt, head;
-    bool q, k;
+    int tt, i;
+    __device__ __forceinline__ void step(int tokens, int rows, int per) {
+        tt += tokens;
+        i += rows;
+        if (i >= per) {
+            i -= per;
+            tt++;
+        }
+    }
 };
-__device__ __forceinline__ RowAt row_at(const AppendArgs& a, int row) {
-    const int per = a.n_heads + 2 * a.n_kv_heads;
-    RowAt r;
-    r.tt = row / per;
-    const int i = row - r.tt * per;
-    r.q = i < a.n_heads;
-    r.k = !r.q && i < a.n_heads + a.n_kv_heads;
-    r.head = r.q ? i : (r.k ? i - a.n_heads : i - a.n_heads - a.n_kv_heads);
-    return r;
-}
 
-__device__ __forceinline__ void load_row(const AppendArgs& a, int seq, int t0, int row, int c0, float (&x)[8]) {
-    const RowAt r = row_at(a, row);
+__device__ __forceinline__ void load_row(const AppendArgs& a, int seq, int t0, const RowAt& r, int c0, float (&x)[8]) {
     const int64_t t = t0 + r.tt;
-    if (r.q) load8(a.q, seq * a.q_seq_stride + t * a.q_token_stride + static_cast<int64_t>(r.head) * a.d + c0, a.in_f16, x);
-    else load8(r.k ? a.k : a.v, seq * a.kv_seq_stride + t * a.kv_token_stride + static_cast<int64_t>(r.head) * a.d + c0, a.in_f16, x);
+    if (r.i < a.n_heads) {
+        load8(a.q, seq * a.q_seq_stride + t * a.q_token_stride + r.i * a.d + c0, a.in_f16, x);
+    } else {
+        const int h = r.i - a.n_heads;
+        const bool k = h < a.n_kv_heads;
+        load8(k ? a.k : a.v, seq * a.kv_seq_stride + t * a.kv_token_stride + (k ? h : h - a.n_kv_heads) * a.d + c0, a.in_f16, x);
+    }
 }
 
-// kKind: alpaca_cache_kind. LP: lanes per row.
+// Position of pair i in the (cos, sin) table. Split halves: a lane reads pairs 8 j .. 8 j + 7 as two 16-byte pieces; the
+// first pieces of all lanes lie together, then the second ones, so that a row's lanes read consecutive banks.
+__device__ __forceinline__ int table_at(int i, int half, int interleaved) {
+    return interleaved ? i : ((i >> 2) & 1) * (half / 2) + (i >> 3) * 4 + (i & 3);
+}
+
+// kKind: alpaca_cache_kind. LP: lanes per row. qw / kw: this lane's norm weights.
 template <int LP, int kKind>
-__device__ __forceinline__ void finish_row(const AppendArgs& a, int seq, int t0, int pos0, int row, bool active, int j,
-                                           const float* s_cos, const float* s_sin, float (&x)[8]) {
-    const RowAt r = row_at(a, active ? row : 0);
+__device__ __forceinline__ void finish_row(const AppendArgs& a, int seq, int t0, int pos0, const RowAt& r, bool active, int j,
+                                           const float* s_cos, const float* s_sin, const float (&qw)[8], const float (&kw)[8],
+                                           float (&x)[8]) {
     const int half = a.d / 2, c0 = 8 * j;
-    const float* w = r.q ? a.q_norm : (r.k ? a.k_norm : nullptr);
-    if (a.q_norm || a.k_norm) {  // the same for the whole grid: every lane takes part in the shuffles
+    const bool is_q = r.i < a.n_heads, is_k = !is_q && r.i < a.n_heads + a.n_kv_heads;
+    const bool norm = active && (is_q ? a.q_norm != nullptr : (is_k && a.k_norm != nullptr));
+    if (__any_sync(0xffffffffu, norm)) {
         float ss = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; e++) ss = fmaf(x[e], x[e], ss);
 #pragma unroll
         for (int o = LP / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (w && active) {
-            const float inv = 1.f / sqrtf(ss / static_cast<float>(a.d) + a.eps);
-            const float4 w0 = *reinterpret_cast<const float4*>(w + c0), w1 = *reinterpret_cast<const float4*>(w + c0 + 4);
-            const float wv[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+        if (norm) {
+            // 1 / sqrt(mean + eps): the hardware's approximation and one Newton step
+            const float m = fmaf(ss, a.inv_d, a.eps), y = rsqrtf(m);
+            const float inv = fmaf(y * 0.5f, fmaf(-m * y, y, 1.f), y);
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = __fmul_rn(__fmul_rn(x[e], inv), wv[e]);
+            for (int e = 0; e < 8; e++) x[e] = __fmul_rn(__fmul_rn(x[e], inv), is_q ? qw[e] : kw[e]);
         }
     }
-    const bool rotate = active && (r.q || r.k);
-    if (a.interleaved) {
-        if (rotate) {
-            const float4 c = *reinterpret_cast<const float4*>(s_cos + r.tt * half + c0 / 2);
-            const float4 s = *reinterpret_cast<const float4*>(s_sin + r.tt * half + c0 / 2);
-            const float cv[4] = {c.x, c.y, c.z, c.w}, sv[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float x0 = x[2 * e], x1 = x[2 * e + 1];
-                x[2 * e] = __fsub_rn(__fmul_rn(x0, cv[e]), __fmul_rn(x1, sv[e]));
-                x[2 * e + 1] = __fadd_rn(__fmul_rn(x0, sv[e]), __fmul_rn(x1, cv[e]));
-            }
-        }
-    } else {
-        // channel i pairs with i + d/2: the lane d/16 further on holds the partners of this lane's eight channels
-        const int lane = threadIdx.x & 31, hl = a.d / 16;
-        const bool first = j < hl;
-        const int other = active ? (first ? lane + hl : lane - hl) : lane;
-        float p[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) p[e] = __shfl_sync(0xffffffffu, x[e], other);
-        if (rotate) {
-            const int i0 = r.tt * half + (first ? c0 : c0 - half);
-#pragma unroll
-            for (int e4 = 0; e4 < 8; e4 += 4) {
-                const float4 c = *reinterpret_cast<const float4*>(s_cos + i0 + e4);
-                const float4 s = *reinterpret_cast<const float4*>(s_sin + i0 + e4);
+    const bool rotate = active && (is_q || is_k);
+    if (__any_sync(0xffffffffu, rotate)) {
+        const float* cs = s_cos + r.tt * half;
+        const float* sn = s_sin + r.tt * half;
+        if (a.interleaved) {
+            if (rotate) {
+                const float4 c = *reinterpret_cast<const float4*>(cs + c0 / 2);
+                const float4 s = *reinterpret_cast<const float4*>(sn + c0 / 2);
                 const float cv[4] = {c.x, c.y, c.z, c.w}, sv[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const float own = x[e4 + e], par = p[e4 + e];
-                    x[e4 + e] = first ? __fsub_rn(__fmul_rn(own, cv[e]), __fmul_rn(par, sv[e]))
-                                      : __fadd_rn(__fmul_rn(par, sv[e]), __fmul_rn(own, cv[e]));
+                    const float x0 = x[2 * e], x1 = x[2 * e + 1];
+                    x[2 * e] = __fsub_rn(__fmul_rn(x0, cv[e]), __fmul_rn(x1, sv[e]));
+                    x[2 * e + 1] = __fadd_rn(__fmul_rn(x0, sv[e]), __fmul_rn(x1, cv[e]));
+                }
+            }
+        } else {
+            // channel i pairs with i + d/2: the lane d/16 further on holds the partners of this lane's eight channels.
+            // first: x c - partner s; second: partner s + x c. One sign covers both.
+            const int lane = threadIdx.x & 31, hl = a.d / 16;
+            const bool first = j < hl;
+            const int other = active ? (first ? lane + hl : lane - hl) : lane;
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) p[e] = __shfl_sync(0xffffffffu, x[e], other);
+            if (rotate) {
+                const int at = 4 * (first ? j : j - hl);
+#pragma unroll
+                for (int e4 = 0; e4 < 2; e4++) {
+                    const float4 c = *reinterpret_cast<const float4*>(cs + at + e4 * (half / 2));
+                    const float4 s = *reinterpret_cast<const float4*>(sn + at + e4 * (half / 2));
+                    const float cv[4] = {c.x, c.y, c.z, c.w}, sv[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float ps = __fmul_rn(p[4 * e4 + e], sv[e]);
+                        x[4 * e4 + e] = __fadd_rn(__fmul_rn(x[4 * e4 + e], cv[e]), first ? -ps : ps);
+                    }
                 }
             }
         }
     }
     float lo = 0.f, hi = 0.f;
-    if (kKind == ALPACA_CACHE_KV4) {  // block extremes, with 0 in the range: four lanes hold a block
+    if (kKind == ALPACA_CACHE_KV4 && __any_sync(0xffffffffu, active && !is_q)) {
+        // block extremes, with 0 in the range: four lanes hold a block
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             lo = min_nan(lo, x[e]);
@@ -184,28 +197,33 @@ __device__ __forceinline__ void finish_row(const AppendArgs& a, int seq, int t0,
     }
     if (!active) return;
     const int64_t t = t0 + r.tt;
-    if (r.q) {
-        store8(a.q_out, seq * a.out_seq_stride + t * a.out_token_stride + static_cast<int64_t>(r.head) * a.d + c0, a.out_f16, x);
+    if (is_q) {
+        store8(a.q_out, seq * a.out_seq_stride + t * a.out_token_stride + r.i * a.d + c0, a.out_f16, x);
         return;
     }
-    const int pos = pos0 + r.tt;
+    const int pos = pos0 + r.tt, head = r.i - a.n_heads - (is_k ? 0 : a.n_kv_heads);
     if (kKind == ALPACA_CACHE_KV4) {
         int64_t unit;
         int ur;
         if (!kv4_locate(a.kv4, seq, pos, a.err, unit, ur)) return;
-        float step, zero;
-        const uint32_t header = kv4_header(lo, hi, step, zero);
-        uint32_t word = 0;
+        const Kv4Block q = kv4_block(lo, hi);
+        if (q.wide) {  // keep quotients in the range of the integer rounding; the codes end at 0 and 15 long before
 #pragma unroll
-        for (int e = 0; e < 8; e++) word |= kv4_code(x[e], step, zero) << (4 * e);
+            for (int e = 0; e < 8; e++) x[e] = fminf(fmaxf(x[e], -32.f * kKv4MaxStep), 32.f * kKv4MaxStep);
+        }
+        uint32_t word = 0;
+        if (q.step > 0.f) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) word += kv4_code(x[e], q) << (4 * e);
+        }
         const int nb = a.d / 32, b = j >> 2, tw = j & 3;
-        uint8_t* codes = (r.k ? a.kv4.k_codes : a.kv4.v_codes) + unit * a.kv4.code_unit_stride +
-                         r.head * a.kv4.code_head_stride + static_cast<int64_t>(ur) * (a.d / 2);
+        uint8_t* codes = (is_k ? a.kv4.k_codes : a.kv4.v_codes) + unit * a.kv4.code_unit_stride +
+                         head * a.kv4.code_head_stride + static_cast<int64_t>(ur) * (a.d / 2);
         *reinterpret_cast<uint32_t*>(codes + 4 * (tw * nb + b)) = word;
         if (tw == 0) {
-            uint16_t* scales = (r.k ? a.kv4.k_scales : a.kv4.v_scales) + unit * a.kv4.scale_unit_stride +
-                               r.head * a.kv4.scale_head_stride + static_cast<int64_t>(ur) * nb;
-            scales[b] = static_cast<uint16_t>(header);
+            uint16_t* scales = (is_k ? a.kv4.k_scales : a.kv4.v_scales) + unit * a.kv4.scale_unit_stride +
+                               head * a.kv4.scale_head_stride + static_cast<int64_t>(ur) * nb;
+            scales[b] = static_cast<uint16_t>(q.header);
         }
     } else {
         int64_t off;
@@ -224,53 +242,62 @@ __device__ __forceinline__ void finish_row(const AppendArgs& a, int seq, int t0,
             }
             off = static_cast<int64_t>(blk) * a.block_stride + static_cast<int64_t>(pos - b * a.block_rows) * a.cache_row_stride;
         }
-        store8(r.k ? a.k_cache : a.v_cache, off + static_cast<int64_t>(r.head) * a.d + c0, kKind == ALPACA_CACHE_F16, x);
+        store8(is_k ? a.k_cache : a.v_cache, off + static_cast<int64_t>(head) * a.d + c0, kKind == ALPACA_CACHE_F16, x);
     }
 }
 
 template <int LP, int kKind>
-__global__ void __launch_bounds__(kAppendThreads) qkv_append_kernel(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, 3) qkv_append_kernel(const __grid_constant__ AppendArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ __align__(16) float s_table[];  // cos [tpc][d/2], sin [tpc][d/2]
     const int t0 = blockIdx.x * a.tpc, seq = blockIdx.y, tid = threadIdx.x;
     const int ntok = min(a.tpc, a.tokens - t0), half = a.d / 2;
-    const int total = ntok * (a.n_heads + 2 * a.n_kv_heads);
     float* s_cos = s_table;
     float* s_sin = s_table + a.tpc * half;
     constexpr int RP = kAppendThreads / LP;  // rows per pass of the CTA
-    const int sub = tid / LP, j = tid % LP;
+    const int sub = tid / LP, j = tid % LP, per = a.n_heads + 2 * a.n_kv_heads;
+    const int step_tokens = RP / per, step_rows = RP - step_tokens * per;
     const bool in = 8 * j < a.d;  // lanes past the row (d not a power of two) only take part in the shuffles
     const auto table = [&](int pos0) {
         for (int i = tid; i < ntok * half; i += kAppendThreads) {
-            const int tt = i / half;
+            const int tt = i / half, at = tt * half + table_at(i - tt * half, half, a.interleaved);
             double sn, cs;
             sincos(static_cast<double>(pos0 + tt) * a.freq[i - tt * half], &sn, &cs);
-            s_cos[i] = static_cast<float>(cs);
-            s_sin[i] = static_cast<float>(sn);
+            s_cos[at] = static_cast<float>(cs);
+            s_sin[at] = static_cast<float>(sn);
         }
     };
     // A uniform start needs no global data: its table is computed while the previous kernel drains.
     if (!a.positions) table(a.start + t0);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int pos0 = (a.positions ? a.positions[seq] : a.start) + t0;
+    float qw[8], kw[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) qw[e] = kw[e] = 1.f;
+    if (in && a.q_norm) load8(a.q_norm, 8 * j, 0, qw);
+    if (in && a.k_norm) load8(a.k_norm, 8 * j, 0, kw);
+    RowAt r;
+    r.tt = sub / per;
+    r.i = sub - r.tt * per;
     float x[kAppendBatch][8];
-    for (int base = 0; base < total; base += RP * kAppendBatch) {
+    const int passes = (ntok * per + RP * kAppendBatch - 1) / (RP * kAppendBatch);
+    for (int p = 0; p < passes; p++) {
+        RowAt at[kAppendBatch];
 #pragma unroll
         for (int b = 0; b < kAppendBatch; b++) {
-            const int row = base + b * RP + sub;
+            at[b] = r;
+            r.step(step_tokens, step_rows, per);
 #pragma unroll
             for (int e = 0; e < 8; e++) x[b][e] = 0.f;
-            if (in && row < total) load_row(a, seq, t0, row, 8 * j, x[b]);
+            if (in && at[b].tt < ntok) load_row(a, seq, t0, at[b], 8 * j, x[b]);
         }
-        if (base == 0) {
+        if (p == 0) {
             if (a.positions) table(pos0);
-            __syncthreads();  // once: `base` is the same in every thread
+            __syncthreads();  // once, by every thread
         }
 #pragma unroll
-        for (int b = 0; b < kAppendBatch; b++) {
-            const int row = base + b * RP + sub;
-            finish_row<LP, kKind>(a, seq, t0, pos0, row, in && row < total, j, s_cos, s_sin, x[b]);
-        }
+        for (int b = 0; b < kAppendBatch; b++)
+            finish_row<LP, kKind>(a, seq, t0, pos0, at[b], in && at[b].tt < ntok, j, s_cos, s_sin, qw, kw, x[b]);
     }
 }
 
@@ -286,7 +313,8 @@ cudaError_t launch_append(const AppendArgs& a, int kind, const cudaLaunchConfig_
 // ------------------------------------------------------------------------------------------------ read back
 
 constexpr int kReadThreads = 256;
-constexpr int kReadBatch = 4;  // words in flight per thread
+constexpr int kReadBatch = 2;  // head rows in flight per lane group
+constexpr int kReadRows = kReadThreads / 4 * kReadBatch;  // head rows per CTA
 
 struct ReadArgs {
     Kv4View c;
@@ -301,10 +329,12 @@ struct ReadArgs {
     unsigned* err;
 };
 
+// NB = d / 32. Four lanes hold a head row, lane t the words t * NB .. of all blocks: channels 32 b + 8 t .. + 7.
+template <int NB>
 __global__ void __launch_bounds__(kReadThreads) kv4_read_kernel(const __grid_constant__ ReadArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int seq = blockIdx.y, nb = a.d / 32, lpr = a.d / 8, per_row = a.n_kv_heads * lpr;
+    const int seq = blockIdx.y, t = threadIdx.x & 3;
     const uint8_t* codes = blockIdx.z ? a.c.v_codes : a.c.k_codes;
     const uint16_t* scales = blockIdx.z ? a.c.v_scales : a.c.k_scales;
     void* out = blockIdx.z ? a.v_out : a.k_out;
@@ -314,40 +344,62 @@ __global__ void __launch_bounds__(kReadThreads) kv4_read_kernel(const __grid_con
         const int64_t n = static_cast<int64_t>(a.q_offsets[seq + 1]) - a.q_offsets[seq];
         rows = n > 0 ? static_cast<int>(max(min(a.start_positions[seq] + n, static_cast<int64_t>(a.n_rows)), static_cast<int64_t>(0))) : 0;
     }
-    const int64_t total = static_cast<int64_t>(rows) * per_row;
-    const int64_t i0 = static_cast<int64_t>(blockIdx.x) * (kReadThreads * kReadBatch) + threadIdx.x;
-    uint32_t w[kReadBatch], h[kReadBatch];
+    uint32_t w[kReadBatch][NB], h[kReadBatch][NB];
     int64_t at[kReadBatch];
 #pragma unroll
     for (int b = 0; b < kReadBatch; b++) {
-        const int64_t i = i0 + b * kReadThreads;
+        const int64_t i = static_cast<int64_t>(blockIdx.x) * kReadRows + b * (kReadThreads / 4) + threadIdx.x / 4;
+        const int row = static_cast<int>(i / a.n_kv_heads), head = static_cast<int>(i - static_cast<int64_t>(row) * a.n_kv_heads);
         at[b] = -1;
-        w[b] = h[b] = 0;
-        if (i < total) {
-            const int row = static_cast<int>(i / per_row), rem = static_cast<int>(i - static_cast<int64_t>(row) * per_row);
-            const int head = rem / lpr, j = rem - head * lpr;
-            at[b] = seq * a.out_seq_stride + row * a.out_row_stride + static_cast<int64_t>(head) * a.d + 8 * j;
-            int64_t unit;
-            int ur;
-            if (kv4_locate(a.c, seq, start + row, a.err, unit, ur)) {  // else the row reads as zero
-                w[b] = *reinterpret_cast<const uint32_t*>(codes + unit * a.c.code_unit_stride + head * a.c.code_head_stride +
-                                                          static_cast<int64_t>(ur) * (a.d / 2) + 4 * ((j & 3) * nb + (j >> 2)));
-                h[b] = scales[unit * a.c.scale_unit_stride + head * a.c.scale_head_stride + static_cast<int64_t>(ur) * nb + (j >> 2)];
+#pragma unroll
+        for (int k = 0; k < NB; k++) w[b][k] = h[b][k] = 0;
+        if (row >= rows) continue;
+        at[b] = seq * a.out_seq_stride + row * a.out_row_stride + head * (32 * NB) + 8 * t;
+        int64_t unit;
+        int ur;
+        if (!kv4_locate(a.c, seq, start + row, a.err, unit, ur)) continue;  // reads as zero
+        const uint32_t* c = reinterpret_cast<const uint32_t*>(codes + unit * a.c.code_unit_stride + head * a.c.code_head_stride +
+                                                              static_cast<int64_t>(ur) * (16 * NB)) + t * NB;
+        const uint16_t* s = scales + unit * a.c.scale_unit_stride + head * a.c.scale_head_stride + static_cast<int64_t>(ur) * NB;
+        if constexpr (NB % 4 == 0) {
+#pragma unroll
+            for (int k = 0; k < NB; k += 4) {
+                const uint4 u = *reinterpret_cast<const uint4*>(c + k);
+                w[b][k] = u.x; w[b][k + 1] = u.y; w[b][k + 2] = u.z; w[b][k + 3] = u.w;
+                const uint2 v = *reinterpret_cast<const uint2*>(s + k);
+                h[b][k] = v.x & 0xFFFFu; h[b][k + 1] = v.x >> 16; h[b][k + 2] = v.y & 0xFFFFu; h[b][k + 3] = v.y >> 16;
+            }
+        } else if constexpr (NB % 2 == 0) {
+#pragma unroll
+            for (int k = 0; k < NB; k += 2) {
+                const uint2 u = *reinterpret_cast<const uint2*>(c + k);
+                w[b][k] = u.x; w[b][k + 1] = u.y;
+                const uint32_t v = *reinterpret_cast<const uint32_t*>(s + k);
+                h[b][k] = v & 0xFFFFu; h[b][k + 1] = v >> 16;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < NB; k++) {
+                w[b][k] = c[k];
+                h[b][k] = s[k];
             }
         }
     }
 #pragma unroll
     for (int b = 0; b < kReadBatch; b++) {
         if (at[b] < 0) continue;
-        const uint4 u = kv4_word_values(w[b], h[b]);
-        if (a.out_f16) {
-            *reinterpret_cast<uint4*>(static_cast<__half*>(out) + at[b]) = u;
-        } else {
-            float4* o = reinterpret_cast<float4*>(static_cast<float*>(out) + at[b]);
-            const float2 f0 = __half22float2(as_half2(u.x)), f1 = __half22float2(as_half2(u.y));
-            const float2 f2 = __half22float2(as_half2(u.z)), f3 = __half22float2(as_half2(u.w));
-            o[0] = make_float4(f0.x, f0.y, f1.x, f1.y);
-            o[1] = make_float4(f2.x, f2.y, f3.x, f3.y);
+#pragma unroll
+        for (int k = 0; k < NB; k++) {
+            const uint4 u = kv4_word_values(w[b][k], h[b][k]);
+            if (a.out_f16) {
+                *reinterpret_cast<uint4*>(static_cast<__half*>(out) + at[b] + 32 * k) = u;
+            } else {
+                float4* o = reinterpret_cast<float4*>(static_cast<float*>(out) + at[b] + 32 * k);
+                const float2 f0 = __half22float2(as_half2(u.x)), f1 = __half22float2(as_half2(u.y));
+                const float2 f2 = __half22float2(as_half2(u.z)), f3 = __half22float2(as_half2(u.w));
+                o[0] = make_float4(f0.x, f0.y, f1.x, f1.y);
+                o[1] = make_float4(f2.x, f2.y, f3.x, f3.y);
+            }
         }
     }
 }
@@ -382,6 +434,7 @@ cudaError_t launch_qkv_append(const alpaca_qkv_desc& d, unsigned* err, cudaStrea
     a.q_norm = d.q_norm;
     a.k_norm = d.k_norm;
     a.eps = d.eps;
+    a.inv_d = 1.f / static_cast<float>(d.head_dim);
     a.in_f16 = d.in_dtype == ALPACA_F16;
     a.out_f16 = d.q_out_dtype == ALPACA_F16;
     a.interleaved = d.interleaved;
@@ -434,12 +487,20 @@ cudaError_t launch_kv4_read(const alpaca_kv4_read_desc& d, const int* start_posi
     a.d = d.head_dim;
     a.out_f16 = d.out_dtype == ALPACA_F16;
     a.err = err;
-    const int64_t words = static_cast<int64_t>(d.n_rows) * d.n_kv_heads * (d.head_dim / 8);
-    const int64_t per = kReadThreads * kReadBatch;
+    const int64_t rows = static_cast<int64_t>(d.n_rows) * d.n_kv_heads;
     cudaLaunchAttribute attr;
     const cudaLaunchConfig_t cfg =
-        pdl_config(dim3(static_cast<unsigned>((words + per - 1) / per), d.n_seqs, 2), kReadThreads, 0, s, &attr);
-    return cudaLaunchKernelEx(&cfg, kv4_read_kernel, a);
+        pdl_config(dim3(static_cast<unsigned>((rows + kReadRows - 1) / kReadRows), d.n_seqs, 2), kReadThreads, 0, s, &attr);
+    switch (d.head_dim / 32) {
+        case 1: return cudaLaunchKernelEx(&cfg, kv4_read_kernel<1>, a);
+        case 2: return cudaLaunchKernelEx(&cfg, kv4_read_kernel<2>, a);
+        case 3: return cudaLaunchKernelEx(&cfg, kv4_read_kernel<3>, a);
+        case 4: return cudaLaunchKernelEx(&cfg, kv4_read_kernel<4>, a);
+        case 5: return cudaLaunchKernelEx(&cfg, kv4_read_kernel<5>, a);
+        case 6: return cudaLaunchKernelEx(&cfg, kv4_read_kernel<6>, a);
+        case 7: return cudaLaunchKernelEx(&cfg, kv4_read_kernel<7>, a);
+        default: return cudaLaunchKernelEx(&cfg, kv4_read_kernel<8>, a);
+    }
 }
 
 }  // namespace alpaca
