@@ -394,7 +394,7 @@ alpaca_cuda_status validate_qkv(const alpaca_qkv_desc* dp) {
         return fail(ALPACA_CUDA_ERR_INVALID_ARGUMENT, sh);
     };
     if (d.n_seqs < 1 || d.n_seqs > 65535 || d.tokens < 1 || d.n_heads < 0 || d.n_kv_heads < 0 || d.start_position < 0 ||
-        (d.n_heads == 0 && d.n_kv_heads == 0) || d.n_heads > (1 << 20) || d.n_kv_heads > (1 << 20))
+        (d.n_heads == 0 && d.n_kv_heads == 0) || d.n_heads > 65535 || d.n_kv_heads > 65535)
         return bad("shapes");
     if (!kv4_head_dim_ok(d.head_dim)) return bad("headDim must be a multiple of 32 up to 256");
     if (!(d.theta > 0.f) || !std::isfinite(d.theta)) return bad("theta must be finite and > 0");
@@ -411,6 +411,7 @@ alpaca_cuda_status validate_qkv(const alpaca_qkv_desc* dp) {
         if (d.q_token_stride < hq || d.q_out_token_stride < hq || d.q_seq_stride < 0 || d.q_out_seq_stride < 0 ||
             (d.n_seqs > 1 && (d.q_seq_stride == 0 || d.q_out_seq_stride == 0)))
             return bad("q / q_out strides");
+        if (d.q_token_stride > kMaxTokenStride || d.q_out_token_stride > kMaxTokenStride) return bad("q / q_out token stride above 2^27");
         if ((d.q_token_stride * is) % 16 || (d.q_seq_stride * is) % 16 || (d.q_out_token_stride * os) % 16 || (d.q_out_seq_stride * os) % 16)
             return bad("q / q_out strides must be multiples of 16 bytes");
         if (d.q == d.q_out && (d.in_dtype != d.q_out_dtype || d.q_token_stride != d.q_out_token_stride || d.q_seq_stride != d.q_out_seq_stride))
@@ -420,6 +421,7 @@ alpaca_cuda_status validate_qkv(const alpaca_qkv_desc* dp) {
     const int64_t hk = static_cast<int64_t>(d.n_kv_heads) * d.head_dim;
     if (!d.k || !d.v || !aligned16(d.k) || !aligned16(d.v)) return bad("k / v null or not 16-byte aligned");
     if (d.kv_token_stride < hk || d.kv_seq_stride < 0 || (d.n_seqs > 1 && d.kv_seq_stride == 0)) return bad("k / v strides");
+    if (d.kv_token_stride > kMaxTokenStride) return bad("k / v token stride above 2^27");
     if ((d.kv_token_stride * is) % 16 || (d.kv_seq_stride * is) % 16) return bad("k / v strides must be multiples of 16 bytes");
     const int64_t rows = d.positions ? 0 : static_cast<int64_t>(d.start_position) + d.tokens;
     if (d.cache_kind == ALPACA_CACHE_KV4) return validate_kv4_cache(d.kv4, d.n_seqs, d.n_kv_heads, d.head_dim, rows, "qkv");

@@ -52,6 +52,7 @@ size_t prefill_workspace_min_bytes(const alpaca_attn_desc& d);
 cudaError_t launch_prefill(const Call& c, cudaStream_t s);
 
 // ---- 4-bit KV cache (kv4_cache.cu, attn_kv4.cu)
+constexpr int64_t kMaxTokenStride = int64_t(1) << 27;  // elements: a CTA's tokens are addressed with 32-bit offsets
 cudaError_t launch_qkv_append(const alpaca_qkv_desc& d, unsigned* err, cudaStream_t s);
 // start_positions / q_offsets: a ragged prefill's (each sequence's visible rows only), or null
 cudaError_t launch_kv4_read(const alpaca_kv4_read_desc& d, const int* start_positions, const int* q_offsets, unsigned* err,

@@ -128,26 +128,31 @@ __device__ __forceinline__ Kv4Block kv4_block(float lo, float hi) {
     b.wide = false;
     b.header = kKv4NanHeader;
     if (!(hi <= FLT_MAX && lo >= -FLT_MAX)) return b;
-    const float s = (hi - lo) / 15.f;
-    b.wide = s >= kKv4MaxStep;
+    const float span = hi - lo, s0 = span * (1.f / 15.f);
+    const float s = __fmaf_rn(__fmaf_rn(-s0, 15.f, span), 1.f / 15.f, s0);  // span / 15 (as in kv4_code_pair); NaN past f32
+    b.wide = !(s < kKv4MaxStep);
     const uint32_t bits = (static_cast<uint32_t>(__half_as_ushort(__float2half_ru(fminf(s, kKv4MaxStep)))) + 15u) & kKv4StepMask;
     b.header = bits;
     if (bits == 0) return b;
     b.step = __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
-    b.inv = 1.f / b.step;
-    const int zero = min(static_cast<int>(rintf(-lo / b.step)), 15);
+    b.inv = __frcp_rn(b.step);
+    const float z0 = -fmaxf(lo, -32.f * kKv4MaxStep) * b.inv;
+    const float z = __fmaf_rn(__fmaf_rn(-z0, b.step, -fmaxf(lo, -32.f * kKv4MaxStep)), b.inv, z0);
+    const int zero = min(__float_as_int(__fadd_rn(z, 12582912.f)) - 0x4B400000, 15);
     b.header = bits | static_cast<uint32_t>(zero);
     b.bias = zero - 0x4B400000;
     return b;
 }
 
-// clamp(round(x / step) + zero, 0, 15), the quotient as f32 division rounds it: from the correctly rounded reciprocal, one
-// residual step gives the correctly rounded quotient (Markstein, "Computation of elementary functions on the IBM RISC
-// System/6000 processor", 1990). Adding 1.5 * 2^23 rounds to an integer, ties to even, and leaves it in the low bits.
-__device__ __forceinline__ uint32_t kv4_code(float x, const Kv4Block& b) {
-    const float q = __fmul_rn(x, b.inv);
-    const float quotient = __fmaf_rn(__fmaf_rn(-q, b.step, x), b.inv, q);
-    return static_cast<uint32_t>(__vimin_s32_relu(__float_as_int(__fadd_rn(quotient, 12582912.f)) + b.bias, 15));
+// clamp(round(x / step) + zero, 0, 15) of two values, the quotient as f32 division rounds it: from the correctly rounded
+// reciprocal, one residual step gives the correctly rounded quotient (Markstein, "Computation of elementary functions on the
+// IBM RISC System/6000 processor", 1990). Adding 1.5 * 2^23 rounds to an integer, ties to even, and leaves it in the low bits.
+__device__ __forceinline__ uint32_t kv4_code_pair(float2 x, const Kv4Block& b) {  // second code in bits 4-7
+    const float2 inv = make_float2(b.inv, b.inv), minus_step = make_float2(-b.step, -b.step);
+    const float2 q = __fmul2_rn(x, inv);
+    const float2 m = __fadd2_rn(__ffma2_rn(__ffma2_rn(q, minus_step, x), inv, q), make_float2(12582912.f, 12582912.f));
+    return static_cast<uint32_t>(__vimin_s32_relu(__float_as_int(m.x) + b.bias, 15)) +
+           16u * static_cast<uint32_t>(__vimin_s32_relu(__float_as_int(m.y) + b.bias, 15));
 }
 
 }  // namespace alpaca

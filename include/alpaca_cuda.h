@@ -345,15 +345,17 @@ typedef enum alpaca_cache_kind {
 
 /* One pass over the new tokens' projections: every query and key head is RMS-normalised over head_dim (where its norm
  * weight is given: x * (1 / sqrt(mean(x^2) + eps)) * w, f32), queries and keys are rotated as alpaca_rope_kv_append
- * rotates them (without norms the results equal that call's bit for bit), queries go to q_out, and rotated keys and raw
- * values to the cache rows of their positions: token t of sequence s at (positions ? positions[s] : start_position) + t.
+ * rotates them (angles, cos and sin in double, rounded once to f32; products rounded separately), queries go to q_out, and
+ * rotated keys and raw values to the cache rows of their positions: token t of sequence s at
+ * (positions ? positions[s] : start_position) + t.
  * A position outside the cache, or a table entry outside the pool, writes no cache row and is reported by
  * alpaca_cuda_device_status; its queries are still written.
- * q_out may be q itself (same type and strides). Pointers 16-byte aligned, strides in elements and multiples of 16 bytes. */
+ * q_out may be q itself (same type and strides). Pointers 16-byte aligned, strides in elements and multiples of 16 bytes,
+ * token strides at most 2^27 elements. */
 typedef struct alpaca_qkv_desc {
     int32_t n_seqs;           /* 1 .. 65535 */
-    int32_t n_heads;          /* query heads (0: no queries) */
-    int32_t n_kv_heads;       /* KV heads (0: no append) */
+    int32_t n_heads;          /* query heads, <= 65535 (0: no queries) */
+    int32_t n_kv_heads;       /* KV heads, <= 65535 (0: no append) */
     int32_t head_dim;         /* multiple of 32, 32 .. 256 */
     int32_t tokens;           /* new tokens per sequence, >= 1 */
     int32_t start_position;   /* position of token 0 when positions is NULL, >= 0 */
