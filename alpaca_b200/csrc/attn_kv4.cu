@@ -1,10 +1,10 @@
 // attn_kv4.cu — attention over the 4-bit KV cache (kv4.cuh).
 //
-//   split kernel   one resident wave of warps ("workers"). A unit is one KV head of one sequence with up to 4 NT of its query
-//                  rows (a query row = one head of one token; the G heads of every token of the call share the KV head),
-//                  cut into tiles of 64 (head_dim 64) or 32 (head_dim 128) cache rows; the units' tiles lie in one row and
-//                  every worker takes an equal run of them, with its own ring of bulk copies and its own running softmax.
-//                  A unit inside one run is finished there; the parts of one that crosses runs go to records.
+//   split kernel   one CTA per SM. A unit is one KV head of one sequence with up to 4 NT of its query rows (a query row = one
+//                  head of one token; the G heads of every token of the call share the KV head), cut into tiles of 64
+//                  (head_dim 64) or 32 (head_dim 128) cache rows. The units' tiles lie in one row and are cut into equal
+//                  chunks, each worked off by one warp with its own cp.async ring and its own running softmax. A unit inside
+//                  one chunk is finished there; the parts of one that crosses chunks go to records.
 //                  Both products run on mma.sync m16n8k16 with the cache as the 16-row operand: S^T = K Q^T (16 keys x 8
 //                  columns) and O^T = V^T P^T (16 channels x 8 columns). A column pair is one query row: f16 high part and
 //                  f16 remainder of q or p, so the f32 sum of the pair's two accumulators carries ~22 bits. Scores,
@@ -12,7 +12,7 @@
 //                  K: codes enter as f16 denormals (c * 2^-24, one AND per pair; codes in bits 4-7 count 16 times, which
 //                  the queries' halves undo), exact; a block's step and zero point are applied to the block's partial
 //                  score in f32: s = sum_b step_b (acc_b - zero_b * qsum_b).
-//                  V: (c - zero) * step is exact in f16 (kv4.cuh), decoded for two keys side by side.
+//                  V: ldmatrix with transposition sets two keys' codes side by side; (c - zero) * step is exact in f16 (kv4.cuh).
 //                  P moves from accumulator to operand layout with movmatrix (no shared memory).
 //   combine        one CTA per query row: rescales the parts' (m, l, acc) records to the common maximum and normalises.
 //   general kernel fp32 SIMT, any head_dim that is a multiple of 32 up to 256: one warp per query row.
@@ -26,8 +26,6 @@
 namespace alpaca {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = 32 * kWarps;
 constexpr int kStages = 2;          // tiles in a warp's ring
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPShift = 7.f;      // p is held times 2^7: its f16 remainder then keeps small p to 2^-31 of the maximum
@@ -43,8 +41,9 @@ struct Kv4Args {
     const int* ctx_lens;
     int uniform_len, max_len;
     int n_seqs, n_heads, n_kv_heads, tokens, group, q_rows, q_groups;  // q_rows = tokens * group per KV head
-    int64_t* plan;   // [0] tiles per worker, [1 + unit] first tile of the unit
-    float* partial;  // [worker][2][query row of the group][d + 4]: accumulators, m (log2 units), l
+    int2* plan;      // [unit]: the first chunk that holds tiles of it, and how many do
+    float* partial;  // [chunk + unit][query row of the group][d + 4]: accumulators, m (log2 units), l
+    int chunks;
     float scale;
     unsigned* err;
 };
@@ -75,25 +74,38 @@ struct Kv4Geo {
     static constexpr int TK = 4096 / D;           // rows of a tile
     static constexpr int GR = TK / 16;            // 16-row groups of a tile
     static constexpr int CROW = D / 2;            // code bytes of a row
+    static constexpr int CPR = CROW / 16;         // 16-byte chunks of a row's codes
     static constexpr int HROW = D / 16;           // header bytes of a row
     static constexpr int CB = TK * CROW;          // 2048
     static constexpr int HB = TK * HROW;          // 256
     static constexpr int STAGE = 2 * (CB + HB);   // K codes, V codes, K headers, V headers
-    static constexpr int WX = D / 64;             // V words per lane and row
     static constexpr int REC = D + 4;             // floats of a partial record
     static constexpr int DEC = 2048;              // bytes of a warp's decoded headers: 1 KB for K, 1 KB for V
     static constexpr int WARP = kStages * STAGE + DEC;
-    // Entry of block b of key pair t of 8-row half `half8` of a tile. The two blocks that a quarter warp reads at once (b = 0, 1
-    // at head_dim 64; x and x + 2 at 128) are adjacent, so the 16-byte reads fall in different banks.
-    __host__ __device__ static constexpr int vd_index(int half8, int b, int t) {
-        return D == 64 ? (half8 * 2 + b) * 4 + t : ((half8 * 2 + (b & 1)) * 2 + (b >> 1)) * 4 + t;
+    // Chunk of V row `row` in shared memory: eight rows' chunks of one index lie in different banks for ldmatrix.
+    __device__ static constexpr int v_chunk(int row, int c) { return D == 64 ? c ^ ((row >> 2) & 1) : c ^ ((row >> 1) & 3); }
+    // Block that lane group g decodes in V (of every 16-byte chunk), and the first of the four channels it holds of chunk c.
+    __device__ static constexpr int v_block(int g) { return (g >> 1) & (NB - 1); }
+    __device__ static constexpr int v_channel(int g, int c) {
+        return D == 64 ? 32 * ((g >> 1) & 1) + 8 * (2 * c + (g >> 2)) + 4 * (g & 1) : 32 * (g >> 1) + 8 * c + 4 * (g & 1);
     }
 };
 
-// Untiled bulk copy global -> shared completing `bytes` on `bar` (16-byte aligned ends and size; no multicast).
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
-                 "r"(bytes), "r"(smem_u32(bar))
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t src_bytes) {  // the rest reads as zero
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
                  : "memory");
 }
 
@@ -117,228 +129,278 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
     return r;
 }
-// x and y each as f16 value (low half) and the f16 of what that leaves (high half): x in r0, y in r1.
+// x and y each as a high part of 11 bits (low half) and the f16 of what that leaves (high half): x in r0, y in r1.
 __device__ __forceinline__ void split_f16_pair(float x, float y, uint32_t& r0, uint32_t& r1) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
-    r0 = __byte_perm(as_u32(h), as_u32(l), 0x5410);
-    r1 = __byte_perm(as_u32(h), as_u32(l), 0x7632);
+    const float hx = __uint_as_float(__float_as_uint(x) & 0xFFFFE000u), hy = __uint_as_float(__float_as_uint(y) & 0xFFFFE000u);
+    r0 = pack_half2(hx, x - hx);
+    r1 = pack_half2(hy, y - hy);
 }
 
-// Starts the copies of rows [row0, min(row0 + TK, row_end)) of one KV head into a stage (one lane). A tile is one run of
-// bytes per plane, or one per pool block it touches; headers are copied in multiples of 16 bytes (rows up to the next
-// multiple of 4, which the cache's 16-row granularity covers) and the surplus is ignored by the reader. A table entry
-// outside the pool reads as zero: its rows' headers are cleared.
+// A lane's places in a head's rows: where its 16 bytes of a tile come from (row 0 of a contiguous cache) and go to.
+struct TileCopy {
+    const uint8_t* k;
+    const uint8_t* v;
+    const uint8_t* h;  // lanes 0-15 K headers, 16-31 V headers
+    uint32_t k_dst, v_dst, h_dst;  // offsets in a stage
+};
 template <int D>
-__device__ __forceinline__ void load_tile(const Kv4Args& a, int seq, int kvh, int row0, int row_end, uint8_t* stage, uint64_t* bar) {
+__device__ __forceinline__ TileCopy tile_copy(const Kv4Args& a, int64_t unit, int kvh, int lane) {
     using Ge = Kv4Geo<D>;
-    const int n = min(Ge::TK, row_end - row0);
-    const uint32_t st = smem_u32(stage);
-    if (!a.c.block_table) {
-        const int64_t code = seq * a.c.code_unit_stride + kvh * a.c.code_head_stride + static_cast<int64_t>(row0) * Ge::CROW;
-        const int64_t scale = seq * a.c.scale_unit_stride + kvh * a.c.scale_head_stride + static_cast<int64_t>(row0) * Ge::NB;
-        const uint32_t cb = n * Ge::CROW, hb = (n * Ge::HROW + 15) & ~15;
-        mbar_arrive_expect_tx(bar, 2 * (cb + hb));
-        bulk_load(st, a.c.k_codes + code, cb, bar);
-        bulk_load(st + 2 * Ge::CB, a.c.k_scales + scale, hb, bar);
-        bulk_load(st + Ge::CB, a.c.v_codes + code, cb, bar);
-        bulk_load(st + 2 * Ge::CB + Ge::HB, a.c.v_scales + scale, hb, bar);
-        return;
+    const int64_t code = unit * a.c.code_unit_stride + kvh * a.c.code_head_stride + 16 * lane;
+    const int64_t scale = unit * a.c.scale_unit_stride + kvh * a.c.scale_head_stride + 8 * (lane & 15);
+    TileCopy c;
+    c.k = a.c.k_codes + code;
+    c.v = a.c.v_codes + code;
+    c.h = reinterpret_cast<const uint8_t*>((lane < 16 ? a.c.k_scales : a.c.v_scales) + scale);
+    c.k_dst = 16 * lane;
+    c.v_dst = Ge::CB + (lane / Ge::CPR) * Ge::CROW + 16 * Ge::v_chunk(lane / Ge::CPR, lane % Ge::CPR);
+    c.h_dst = 2 * Ge::CB + 16 * lane;
+    return c;
+}
+
+// Copies rows [row0, min(row0 + TK, row_end)) of one KV head into a stage. The rows past them, and rows of a table entry
+// outside the pool, read as zero codes with step 0. The caller commits the group.
+template <int D>
+__device__ __forceinline__ void load_tile(const Kv4Args& a, const TileCopy& head, int seq, int kvh, int row0, int row_end, uint32_t stage,
+                                          int lane) {
+    using Ge = Kv4Geo<D>;
+    const int n = row_end - row0;
+    TileCopy c = head;
+    int64_t unit = seq;
+    int r = row0;
+    bool whole = n >= Ge::TK;  // a full tile of one unit: one run of bytes per plane
+    if (a.c.block_table) {
+        whole = whole && a.c.rows % Ge::TK == 0 && kv4_locate(a.c, seq, row0, a.err, unit, r);
+        if (whole) c = tile_copy<D>(a, unit, kvh, lane);
     }
-    uint32_t total = 0;
-    for (int r = 0; r < n;) {  // the copies may land before the barrier expects them: its count stays pending until the arrive
-        const int row = row0 + r, b = row / a.c.rows, in = row - b * a.c.rows, m = min(n - r, a.c.rows - in);
-        const int blk = b < a.c.max_blocks ? a.c.block_table[static_cast<int64_t>(seq) * a.c.max_blocks + b] : -1;
-        const uint32_t cb = m * Ge::CROW, hb = (m * Ge::HROW + 15) & ~15;
-        if (blk >= 0 && blk < a.c.pool_blocks) {
-            const int64_t code = blk * a.c.code_unit_stride + kvh * a.c.code_head_stride + static_cast<int64_t>(in) * Ge::CROW;
-            const int64_t scale = blk * a.c.scale_unit_stride + kvh * a.c.scale_head_stride + static_cast<int64_t>(in) * Ge::NB;
-            bulk_load(st + r * Ge::CROW, a.c.k_codes + code, cb, bar);
-            bulk_load(st + 2 * Ge::CB + r * Ge::HROW, a.c.k_scales + scale, hb, bar);
-            bulk_load(st + Ge::CB + r * Ge::CROW, a.c.v_codes + code, cb, bar);
-            bulk_load(st + 2 * Ge::CB + Ge::HB + r * Ge::HROW, a.c.v_scales + scale, hb, bar);
-            total += 2 * (cb + hb);
-        } else {
-            atomicOr(a.err, kDevErrBadIndex);
-            uint4* h = reinterpret_cast<uint4*>(stage + 2 * Ge::CB + r * Ge::HROW);
-            for (uint32_t i = 0; i < hb / 16; i++) h[i] = h[i + Ge::HB / 16] = make_uint4(0, 0, 0, 0);
-            fence_proxy_async_smem();  // before a later bulk copy into this stage
+    if (whole) {
+        const uint8_t* k = c.k + static_cast<int64_t>(r) * Ge::CROW;
+        const uint8_t* v = c.v + static_cast<int64_t>(r) * Ge::CROW;
+#pragma unroll
+        for (int i = 0; i < Ge::CB / 512; i++) cp_async16(stage + c.k_dst + 512 * i, k + 512 * i);
+        cp_async16(stage + c.h_dst, c.h + static_cast<int64_t>(r) * Ge::HROW);
+#pragma unroll
+        for (int i = 0; i < Ge::CB / 512; i++) cp_async16(stage + c.v_dst + 512 * i, v + 512 * i);
+    } else {  // by 16-row groups, which never leave their unit: lane i finds group i
+        int64_t code = 0, scale = 0;
+        bool ok = false;
+        if (lane < Ge::GR && 16 * lane < n) {
+            ok = kv4_locate(a.c, seq, row0 + 16 * lane, a.err, unit, r);
+            if (ok) {
+                code = unit * a.c.code_unit_stride + kvh * a.c.code_head_stride + static_cast<int64_t>(r) * Ge::CROW;
+                scale = unit * a.c.scale_unit_stride + kvh * a.c.scale_head_stride + static_cast<int64_t>(r) * Ge::NB;
+            }
         }
-        r += m;
+#pragma unroll
+        for (int i = 0; i < Ge::CB / 512; i++) {
+            const int row = lane / Ge::CPR + 32 / Ge::CPR * i, gr = 32 / Ge::CPR * i / 16;
+            const int64_t base = __shfl_sync(0xffffffffu, code, gr);
+            const bool in = __shfl_sync(0xffffffffu, static_cast<int>(ok), gr) && row < n;
+            const int64_t off = base + (in ? (row - 16 * gr) * Ge::CROW + 16 * (lane % Ge::CPR) : 0);
+            cp_async16(stage + c.k_dst + 512 * i, a.c.k_codes + off, in ? 16u : 0u);
+            cp_async16(stage + c.v_dst + 512 * i, a.c.v_codes + off, in ? 16u : 0u);
+        }
+        constexpr int RPC = 16 / Ge::HROW;  // rows per chunk of headers
+        const int row = (lane & 15) * RPC, gr = row / 16;
+        const int64_t base = __shfl_sync(0xffffffffu, scale, gr);
+        const bool in = __shfl_sync(0xffffffffu, static_cast<int>(ok), gr);
+        const int bytes = in ? min(max((n - row) * Ge::HROW, 0), 16) : 0;
+        const uint16_t* scales = lane < 16 ? a.c.k_scales : a.c.v_scales;
+        cp_async16(stage + c.h_dst, scales + base + (bytes > 0 ? (row - 16 * gr) * Ge::NB : 0), static_cast<uint32_t>(bytes));
     }
-    mbar_arrive_expect_tx(bar, total);
 }
 
 // A tile's headers decoded once per warp: per key the (step, zero * 2^-24) of its K blocks in f32, and per pair of keys that
-// meet in a V operand register the pair's Kv4Pair for each block. Rows at or past `n` get step 0.
+// meet in a V operand register (2t, 2t + 1 of eight) the pair's Kv4Pair for each block.
 template <int D>
-__device__ __forceinline__ void decode_headers(const uint8_t* stage, float4* s_kd, uint4* s_vd, int n, int lane) {
+__device__ __forceinline__ void decode_headers(const uint8_t* stage, float4* s_kd, uint4* s_vd, int lane) {
     using Ge = Kv4Geo<D>;
     constexpr int WPK = Ge::NB / 2;  // header words per key
     const uint32_t* kh = reinterpret_cast<const uint32_t*>(stage + 2 * Ge::CB);
     const uint32_t* vh = kh + Ge::HB / 4;
 #pragma unroll
     for (int k = 0; k < Ge::HB / 128; k++) {
-        const int i = lane + 32 * k;
-        const uint32_t h = i / WPK < n ? kh[i] : 0u;
+        const uint32_t h = kh[lane + 32 * k];
         const float2 d = __half22float2(as_half2(h & 0xFFF0FFF0u)), z = __half22float2(as_half2(h & 0x000F000Fu));
-        s_kd[i] = make_float4(d.x, z.x, d.y, z.y);
+        s_kd[lane + 32 * k] = make_float4(d.x, z.x, d.y, z.y);
     }
-    // pair i of the tile: rows 2t, 2t + 1 of half h of group gr (in operand order, see compute_tile); lane's word of it
-    const int pair = lane / WPK, word = lane % WPK, t = pair & 3, base = (pair >> 2) * 8;
-    const int ke = base + ((2 * t) ^ (t >> 1)), ko = base + ((2 * t + 1) ^ (t >> 1));
-    const uint32_t he = ke < n ? vh[ke * WPK + word] : 0u, ho = ko < n ? vh[ko * WPK + word] : 0u;
+    const int pair = lane / WPK, word = lane % WPK;  // keys 2 pair, 2 pair + 1; blocks 2 word, 2 word + 1
+    const uint32_t he = vh[2 * pair * WPK + word], ho = vh[(2 * pair + 1) * WPK + word];
     const Kv4Pair p0 = kv4_pair(__byte_perm(he, ho, 0x5410)), p1 = kv4_pair(__byte_perm(he, ho, 0x7632));
-    s_vd[Kv4Geo<D>::vd_index(pair >> 2, 2 * word, t)] = make_uint4(as_u32(p0.d), as_u32(p0.z), as_u32(p0.d16), as_u32(p0.z16));
-    s_vd[Kv4Geo<D>::vd_index(pair >> 2, 2 * word + 1, t)] = make_uint4(as_u32(p1.d), as_u32(p1.z), as_u32(p1.d16), as_u32(p1.z16));
+    uint4* out = s_vd + ((pair >> 2) * Ge::NB + 2 * word) * 4 + (pair & 3);  // [eight keys][block][pair of them]
+    out[0] = make_uint4(as_u32(p0.d), as_u32(p0.z), as_u32(p0.d16), as_u32(p0.z16));
+    out[4] = make_uint4(as_u32(p1.d), as_u32(p1.z), as_u32(p1.d16), as_u32(p1.z16));
 }
 
-// State of the query rows a lane keeps: nt-th row = 4 nt + lane % 4 of the CTA's group.
-template <int D, int NT>
+// FO: with one or two query rows (and NT = 1) the columns that would stand empty serve other keys. Column pair c then is query
+// row c % (4 / FO) over the 16-row groups gr with gr % FO == c / (4 / FO): a tile's scores, exponentials and their operand
+// conversions shrink FO-fold, the MMAs stay as many (their B operands are zero in the other pairs' columns).
+template <int NT, int FO>
+__host__ __device__ constexpr int query_rows() {
+    return 4 * NT / FO;
+}
+
+// State of the query rows a lane keeps: nt-th row = 4 nt + lane % 4 of the unit's (FO > 1: row lane % 4 % (4 / FO)).
+template <int D, int NT, int FO>
 struct RowState {
+    uint32_t qb[FO][NT][D / 32][4];  // query operands, per fold
     float qsum[NT][D / 32];  // sum of a block's (scaled) queries
     float fs[NT];            // raw score -> log2 units
     float m[NT], thr[NT], negm[NT], l[NT];
     int lim[NT];             // visible rows
-    float o[NT][D / 64][8];  // accumulators of the lane's eight channels per V word
+    float o[NT][D / 32][4];  // accumulators of the lane's four channels per chunk of V codes
 };
 
-template <int D, int NT>
+template <int D, int NT, int FO>
 __device__ __forceinline__ void compute_tile(const uint8_t* st, const float4* s_kd, const uint4* s_vd, int row0, int min_lim,
-                                             const uint32_t (&qb)[NT][D / 32][4], RowState<D, NT>& s, int g, int t) {
+                                             RowState<D, NT, FO>& s, int lane) {
     using Ge = Kv4Geo<D>;
-    constexpr int NB = Ge::NB, GR = Ge::GR, WX = Ge::WX;
-    const uint8_t* s_kc = st;
-    const uint8_t* s_vc = st + Ge::CB;
-    // Rows of a 16-row group in operand order: operand row r < 8 is key r ^ (r >> 2), r >= 8 key 8 more. Any order serves
-    // (keys meet only in sums); this one keeps both the K and the V reads free of bank conflicts.
-    const int kg = g ^ (g >> 2), ke = (2 * t) ^ (t >> 1), ko = (2 * t + 1) ^ (t >> 1);
+    constexpr int NB = Ge::NB, GR = Ge::GR, CPR = Ge::CPR, SG = GR / FO, QP = 4 / FO;  // SG sets of FO groups
+    static_assert(FO == 1 || NT == 1, "folding is for one group of query rows");
+    const int g = lane >> 2, t = lane & 3;
+    const int fold = t / QP, column_fold = (g >> 1) / QP;  // of this lane's scores; of its operand column
 
-    float r[GR][2][NT];
+    float r[SG][2][NT];
 #pragma unroll
-    for (int gr = 0; gr < GR; gr++) {
-        uint32_t w[2][NB];
-        float dk[2][NB], zk[2][NB];
+    for (int sg = 0; sg < SG; sg++) {
+        float acc[NB][NT][4];
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int key = 16 * gr + 8 * h + kg;
-            const uint8_t* p = s_kc + key * Ge::CROW;
-            if (D == 64) {
-                const uint2 u = *reinterpret_cast<const uint2*>(p + 8 * t);
-                w[h][0] = u.x;
-                w[h][1] = u.y;
-            } else {
-                const uint4 u = *reinterpret_cast<const uint4*>(p + 16 * t);
-                w[h][0] = u.x; w[h][1] = u.y; w[h][NB - 2] = u.z; w[h][NB - 1] = u.w;
+        for (int f = 0; f < FO; f++) {
+            uint32_t w[2][NB];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const uint8_t* p = st + (16 * (sg * FO + f) + 8 * h + g) * Ge::CROW + 4 * NB * t;
+                if (D == 64) {
+                    const uint2 u = *reinterpret_cast<const uint2*>(p);
+                    w[h][0] = u.x;
+                    w[h][1] = u.y;
+                } else {
+                    const uint4 u = *reinterpret_cast<const uint4*>(p);
+                    w[h][0] = u.x; w[h][1] = u.y; w[h][NB - 2] = u.z; w[h][NB - 1] = u.w;
+                }
             }
 #pragma unroll
-            for (int i = 0; i < NB / 2; i++) {
-                const float4 u = s_kd[key * (NB / 2) + i];
-                dk[h][2 * i] = u.x; zk[h][2 * i] = u.y; dk[h][2 * i + 1] = u.z; zk[h][2 * i + 1] = u.w;
+            for (int b = 0; b < NB; b++) {
+                const uint32_t a0[4] = {w[0][b] & 0x000F000Fu, w[1][b] & 0x000F000Fu, w[0][b] & 0x00F000F0u, w[1][b] & 0x00F000F0u};
+                const uint32_t x0 = w[0][b] >> 8, x1 = w[1][b] >> 8;
+                const uint32_t a1[4] = {x0 & 0x000F000Fu, x1 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x00F000F0u};
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    if (f == 0) mma16816_first(acc[b][nt], a0, s.qb[f][nt][b][0], s.qb[f][nt][b][1]);
+                    else mma16816(acc[b][nt], a0, s.qb[f][nt][b][0], s.qb[f][nt][b][1]);
+                    mma16816(acc[b][nt], a1, s.qb[f][nt][b][2], s.qb[f][nt][b][3]);
+                }
             }
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) r[gr][0][nt] = r[gr][1][nt] = 0.f;
+        for (int h = 0; h < 2; h++) {
+            const float4* kd = s_kd + (16 * (sg * FO + fold) + 8 * h + g) * (NB / 2);
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-            const uint32_t a0[4] = {w[0][b] & 0x000F000Fu, w[1][b] & 0x000F000Fu, w[0][b] & 0x00F000F0u, w[1][b] & 0x00F000F0u};
-            const uint32_t x0 = w[0][b] >> 8, x1 = w[1][b] >> 8;
-            const uint32_t a1[4] = {x0 & 0x000F000Fu, x1 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x00F000F0u};
+            for (int nt = 0; nt < NT; nt++) r[sg][h][nt] = 0.f;
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                float acc[4];
-                mma16816_first(acc, a0, qb[nt][b][0], qb[nt][b][1]);
-                mma16816(acc, a1, qb[nt][b][2], qb[nt][b][3]);
-                r[gr][0][nt] = fmaf(dk[0][b], fmaf(-zk[0][b], s.qsum[nt][b], acc[0] + acc[1]), r[gr][0][nt]);
-                r[gr][1][nt] = fmaf(dk[1][b], fmaf(-zk[1][b], s.qsum[nt][b], acc[2] + acc[3]), r[gr][1][nt]);
+            for (int i = 0; i < NB / 2; i++) {
+                const float4 u = kd[i];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    r[sg][h][nt] = fmaf(u.x, fmaf(-u.y, s.qsum[nt][2 * i], acc[2 * i][nt][2 * h] + acc[2 * i][nt][2 * h + 1]), r[sg][h][nt]);
+                    r[sg][h][nt] =
+                        fmaf(u.z, fmaf(-u.w, s.qsum[nt][2 * i + 1], acc[2 * i + 1][nt][2 * h] + acc[2 * i + 1][nt][2 * h + 1]), r[sg][h][nt]);
+                }
             }
         }
     }
     if (row0 + Ge::TK > min_lim) {  // some row of the tile is hidden from some query row
 #pragma unroll
-        for (int gr = 0; gr < GR; gr++)
+        for (int sg = 0; sg < SG; sg++)
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
-                    if (row0 + 16 * gr + 8 * h + kg >= s.lim[nt]) r[gr][h][nt] = -INFINITY;
+                    if (row0 + 16 * (sg * FO + fold) + 8 * h + g >= s.lim[nt]) r[sg][h][nt] = -INFINITY;
     }
 
-    uint32_t pb[GR][2][NT];
+    uint32_t pb[SG][2][NT];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
         float mx = r[0][0][nt];
 #pragma unroll
-        for (int gr = 0; gr < GR; gr++) mx = fmax3(mx, r[gr][0][nt], r[gr][1][nt]);
+        for (int sg = 0; sg < SG; sg++) mx = fmax3(mx, r[sg][0][nt], r[sg][1][nt]);
         if (__any_sync(0xffffffffu, mx > s.thr[nt])) {  // the reference maximum moves (rare after the first tile)
 #pragma unroll
-            for (int o = 4; o <= 16; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            for (int o = QP; o <= 16; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
             const float mn = fmaxf(s.m[nt], mx);
             const float alpha = s.m[nt] == -INFINITY ? 0.f : ex2_approx(s.fs[nt] * (s.m[nt] - mn));
             s.l[nt] *= alpha;
 #pragma unroll
-            for (int x = 0; x < WX; x++)
+            for (int c = 0; c < CPR; c++)
 #pragma unroll
-                for (int e = 0; e < 8; e++) s.o[nt][x][e] *= alpha;
+                for (int e = 0; e < 4; e++) s.o[nt][c][e] *= alpha;
             s.m[nt] = mn;
             s.thr[nt] = mn + kMaxSlack / s.fs[nt];
             s.negm[nt] = mn == -INFINITY ? kPShift : kPShift - s.fs[nt] * mn;
         }
 #pragma unroll
-        for (int gr = 0; gr < GR; gr++) {
-            const float p0 = ex2_approx(fmaf(s.fs[nt], r[gr][0][nt], s.negm[nt]));  // hidden rows: 2^-inf = 0
-            const float p1 = ex2_approx(fmaf(s.fs[nt], r[gr][1][nt], s.negm[nt]));
+        for (int sg = 0; sg < SG; sg++) {
+            const float p0 = ex2_approx(fmaf(s.fs[nt], r[sg][0][nt], s.negm[nt]));  // hidden rows: 2^-inf = 0
+            const float p1 = ex2_approx(fmaf(s.fs[nt], r[sg][1][nt], s.negm[nt]));
             s.l[nt] += p0;
             s.l[nt] += p1;
             uint32_t u0, u1;
             split_f16_pair(p0, p1, u0, u1);
-            pb[gr][0][nt] = movmatrix(u0);
-            pb[gr][1][nt] = movmatrix(u1);
+            pb[sg][0][nt] = movmatrix(u0);
+            pb[sg][1][nt] = movmatrix(u1);
         }
     }
 
+    // V: ldmatrix with transposition hands lane (g, t) the four codes that chunk c of rows 2t, 2t + 1 of eight holds at g, the
+    // two rows side by side: one register for four channels of two keys. Matrices: keys 0-7 and 8-15 of chunks c, c + 1.
+    const int v_row = (lane & 7) + 8 * ((lane >> 3) & 1);
+    const uint32_t s_v = smem_u32(st + Ge::CB) + v_row * Ge::CROW;
 #pragma unroll
-    for (int x = 0; x < WX; x++) {
-        float acc[4][NT][4];
-        const int blk = (WX * g + x) % NB;  // block of word WX g + x of a row
+    for (int c = 0; c < CPR; c += 2) {
+        float acc[2][2][NT][4];  // [chunk][channels 0, 1 / 2, 3 in operand rows g, g + 8]
+        const uint32_t addr = s_v + 16 * Ge::v_chunk(v_row, c + (lane >> 4));
 #pragma unroll
         for (int gr = 0; gr < GR; gr++) {
-            uint32_t w[4];
+            uint32_t w[4], b0[NT], b1[NT];
+            ldmatrix_x4_trans(addr + 16 * gr * Ge::CROW, w);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                b0[nt] = FO == 1 || column_fold == gr % FO ? pb[gr / FO][0][nt] : 0u;
+                b1[nt] = FO == 1 || column_fold == gr % FO ? pb[gr / FO][1][nt] : 0u;
+            }
             Kv4Pair p[2];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const uint4 u = s_vd[Ge::vd_index(2 * gr + h, blk, t)];
+                const uint4 u = s_vd[((2 * gr + h) * NB + Ge::v_block(g)) * 4 + t];
                 p[h].d = as_half2(u.x);
                 p[h].z = as_half2(u.y);
                 p[h].d16 = as_half2(u.z);
                 p[h].z16 = as_half2(u.w);
-                const uint8_t* r0 = s_vc + (16 * gr + 8 * h + ke) * Ge::CROW + 4 * (WX * g + x);
-                const uint8_t* r1 = s_vc + (16 * gr + 8 * h + ko) * Ge::CROW + 4 * (WX * g + x);
-                w[2 * h] = *reinterpret_cast<const uint32_t*>(r0);
-                w[2 * h + 1] = *reinterpret_cast<const uint32_t*>(r1);
             }
-            const uint32_t lo0 = __byte_perm(w[0], w[1], 0x5410), hi0 = __byte_perm(w[0], w[1], 0x7632);
-            const uint32_t lo1 = __byte_perm(w[2], w[3], 0x5410), hi1 = __byte_perm(w[2], w[3], 0x7632);
 #pragma unroll
-            for (int m = 0; m < 4; m++) {  // channels 2m and 2m + 1 of the word in operand rows g and g + 8
-                const uint32_t u0 = (m < 2 ? lo0 : hi0) >> (8 * (m & 1)), u1 = (m < 2 ? lo1 : hi1) >> (8 * (m & 1));
-                const uint32_t va[4] = {kv4_lo(u0, p[0]), kv4_hi(u0, p[0]), kv4_lo(u1, p[1]), kv4_hi(u1, p[1])};
+            for (int k = 0; k < 2; k++)
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    if (gr == 0) mma16816_first(acc[m][nt], va, pb[gr][0][nt], pb[gr][1][nt]);
-                    else mma16816(acc[m][nt], va, pb[gr][0][nt], pb[gr][1][nt]);
+                for (int m = 0; m < 2; m++) {
+                    const uint32_t u0 = w[2 * k] >> (8 * m), u1 = w[2 * k + 1] >> (8 * m);
+                    const uint32_t va[4] = {kv4_lo(u0, p[0]), kv4_hi(u0, p[0]), kv4_lo(u1, p[1]), kv4_hi(u1, p[1])};
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        if (gr == 0) mma16816_first(acc[k][m][nt], va, b0[nt], b1[nt]);
+                        else mma16816(acc[k][m][nt], va, b0[nt], b1[nt]);
+                    }
                 }
-            }
         }
         // a tile's sums are added in f32 here: long chains of MMA accumulation lose low bits one way
 #pragma unroll
-        for (int m = 0; m < 4; m++)
+        for (int k = 0; k < 2; k++)
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                s.o[nt][x][2 * m] += acc[m][nt][0] + acc[m][nt][1];
-                s.o[nt][x][2 * m + 1] += acc[m][nt][2] + acc[m][nt][3];
-            }
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    s.o[nt][c + k][2 * m] += acc[k][m][nt][0] + acc[k][m][nt][1];
+                    s.o[nt][c + k][2 * m + 1] += acc[k][m][nt][2] + acc[k][m][nt][3];
+                }
     }
 }
 
@@ -348,77 +410,83 @@ __device__ __forceinline__ int unit_tiles(int L) {
     return max(1, (L + Kv4Geo<D>::TK - 1) / Kv4Geo<D>::TK);
 }
 
-// The work of a call is its units' tiles in one row, sequence by sequence; worker (warp) w takes tiles [w C, (w + 1) C),
-// C = ceil(tiles / workers), so that all workers of the one resident wave end together whatever the contexts are.
-struct Range {
-    int64_t begin, end, chunk;  // tiles
-    int64_t first;              // first tile of the unit that `begin` lies in
-    int seq, head_group;        // that unit: sequence, kv_head * q_groups + query group
-    int L;                      // the sequence's context
+// The work of a call is its units' tiles in one row, sequence by sequence, cut into equal chunks, one per warp: all warps of
+// the one resident wave then have the same number of tiles, whatever the contexts are.
+struct Chunk {
+    int64_t begin, end, size;  // tiles; `size` of every chunk but the last
+    int64_t first;             // first tile of the unit that `begin` lies in
+    int seq, head_group, L;    // that unit: sequence, kv_head * q_groups + query group, the sequence's context
 };
 
 template <int D>
-__device__ __forceinline__ Range find_range(const Kv4Args& a, int64_t worker, int64_t workers, int lane) {
-    Range r;
+__device__ __forceinline__ Chunk find_chunk(const Kv4Args& a, int64_t index, int lane) {
+    Chunk c;
     const int64_t hg = static_cast<int64_t>(a.n_kv_heads) * a.q_groups;
+    constexpr int HELD = 2;  // blocks of 32 contexts kept in registers: one round trip for the usual batches
+    int held[HELD];
     int64_t total = 0;
     if (a.ctx_lens) {
-        for (int s = lane; s < a.n_seqs; s += 32) total += unit_tiles<D>(ctx_of(a, s));
 #pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        for (int i = 0; i < HELD; i++) held[i] = lane + 32 * i < a.n_seqs ? ctx_of(a, lane + 32 * i) : 0;
+#pragma unroll
+        for (int i = 0; i < HELD; i++) total += lane + 32 * i < a.n_seqs ? unit_tiles<D>(held[i]) : 0;
+        for (int s = lane + 32 * HELD; s < a.n_seqs; s += 32) total += unit_tiles<D>(ctx_of(a, s));
+        // a lane's sum is below 2^36: two 32-bit sums hold the warp's
+        const unsigned lo = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(total & 0xFFFFF));
+        const unsigned hi = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(total >> 20));
+        total = (static_cast<int64_t>(hi) << 20) + lo;
     } else {
         total = static_cast<int64_t>(a.n_seqs) * unit_tiles<D>(a.uniform_len);
     }
     total *= hg;
-    r.chunk = (total + workers - 1) / workers;
-    r.begin = worker * r.chunk;
-    r.end = min(r.begin + r.chunk, total);
-    if (r.begin >= r.end) return r;
+    c.size = (total + a.chunks - 1) / a.chunks;
+    c.begin = index * c.size;
+    c.end = min(c.begin + c.size, total);
+    if (c.begin >= c.end) return c;
     if (!a.ctx_lens) {
         const int t = unit_tiles<D>(a.uniform_len);
-        const int64_t unit = r.begin / t;
-        r.first = unit * t;
-        r.seq = static_cast<int>(unit / hg);
-        r.head_group = static_cast<int>(unit - r.seq * hg);
-        r.L = a.uniform_len;
-        return r;
+        const int64_t unit = c.begin / t;
+        c.first = unit * t;
+        c.seq = static_cast<int>(unit / hg);
+        c.head_group = static_cast<int>(unit - c.seq * hg);
+        c.L = a.uniform_len;
+        return c;
     }
-    int64_t before = 0;  // tiles (of all heads) before the chunk of 32 sequences
+    int64_t before = 0;  // tiles before the block of 32 sequences
     for (int s0 = 0;; s0 += 32) {
         const int s = s0 + lane;
-        const int L = s < a.n_seqs ? ctx_of(a, s) : 0;
-        const int64_t mine = s < a.n_seqs ? unit_tiles<D>(L) * hg : 0;
-        int64_t incl = mine;
+        const int L = s0 == 0 ? held[0] : (s0 == 32 ? held[1] : (s < a.n_seqs ? ctx_of(a, s) : 0));
+        const int mine = s < a.n_seqs ? unit_tiles<D>(L) : 0;  // at most 2^25: a block's sum fits 32 bits
+        int incl = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
+            const int x = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += x;
         }
-        const unsigned past = __ballot_sync(0xffffffffu, before + incl > r.begin);
+        const unsigned past = __ballot_sync(0xffffffffu, before + incl * hg > c.begin);
         if (past) {  // begin < total: some sequence holds it
             const int src = __ffs(past) - 1;
-            r.seq = s0 + src;
-            r.L = __shfl_sync(0xffffffffu, L, src);
-            const int64_t start = before + __shfl_sync(0xffffffffu, incl - mine, src);
-            const int t = unit_tiles<D>(r.L);
-            r.head_group = static_cast<int>((r.begin - start) / t);
-            r.first = start + static_cast<int64_t>(r.head_group) * t;
-            return r;
+            c.seq = s0 + src;
+            c.L = __shfl_sync(0xffffffffu, L, src);
+            const int64_t start = before + __shfl_sync(0xffffffffu, incl - mine, src) * hg;
+            const int t = unit_tiles<D>(c.L);
+            c.head_group = static_cast<int>((c.begin - start) / t);
+            c.first = start + static_cast<int64_t>(c.head_group) * t;
+            return c;
         }
-        before += __shfl_sync(0xffffffffu, incl, 31);
+        before += __shfl_sync(0xffffffffu, incl, 31) * hg;
     }
 }
 
 // Query operands of the group's rows r0 .. r0 + 4 NT - 1. Column 2 q + {0, 1} of an operand is query row q's (high part,
 // remainder): lane group g holds row g >> 1 and part g & 1; lane t the channels 32 b + 8 t + .. of every block, in the order of
 // the K codes' nibbles. Rows are scaled by a power of two to [2^10, 2^11) so that neither part leaves f16's normal range.
-template <int D, int NT>
-__device__ __forceinline__ void load_queries(const Kv4Args& a, int seq, int kvh, int r0, int L, uint32_t (&qb)[NT][D / 32][4],
-                                             RowState<D, NT>& s, int g, int t) {
-    constexpr int NB = D / 32;
+template <int D, int NT, int FO>
+__device__ __forceinline__ void load_queries(const Kv4Args& a, int seq, int kvh, int r0, int L, RowState<D, NT, FO>& s, int g, int t) {
+    constexpr int NB = D / 32, QP = 4 / FO;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-        const int rr = r0 + 4 * nt + (g >> 1);
+        const int rr = r0 + 4 * nt + (g >> 1) % QP;
         float x[NB][8];
         float amax = 0.f;
         if (rr < a.q_rows) {
@@ -471,172 +539,181 @@ __device__ __forceinline__ void load_queries(const Kv4Args& a, int seq, int kvh,
             for (int i = 0; i < 4; i++) {  // nibble pair (i, i + 4); codes of odd i count 16 times
                 uint32_t u, v;
                 split_f16_pair(x[b][i] * ((i & 1) ? 0.0625f : 1.f), x[b][i + 4] * ((i & 1) ? 0.0625f : 1.f), u, v);
-                qb[nt][b][i] = __byte_perm(u, v, (g & 1) ? 0x7632 : 0x5410);
+                const uint32_t q = __byte_perm(u, v, (g & 1) ? 0x7632 : 0x5410);
+#pragma unroll
+                for (int f = 0; f < FO; f++) s.qb[f][nt][b][i] = FO == 1 || (g >> 1) / QP == f ? q : 0u;
             }
         }
         s.m[nt] = s.thr[nt] = -INFINITY;
         s.negm[nt] = kPShift;
         s.l[nt] = 0.f;
-        s.lim[nt] = L - a.tokens + 1 + (r0 + 4 * nt + t) / a.group;
+        s.lim[nt] = L - a.tokens + 1 + (r0 + 4 * nt + t % QP) / a.group;
 #pragma unroll
-        for (int x2 = 0; x2 < D / 64; x2++)
+        for (int c = 0; c < D / 32; c++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) s.o[nt][x2][e] = 0.f;
+            for (int e = 0; e < 4; e++) s.o[nt][c][e] = 0.f;
     }
 }
 
-// CTAs per SM that the registers and the shared memory are laid out for (one wave of workers is resident).
-__host__ __device__ constexpr int ctas_per_sm(int D, int NT) { return NT == 4 ? 2 : (NT == 2 ? 3 : (D == 128 ? 4 : 5)); }
+// Warps of a CTA, one CTA per SM: as many as the registers of the form allow (128, 168 and 255 a thread).
+__host__ __device__ constexpr int split_warps(int NT) { return NT == 4 ? 8 : (NT == 2 ? 12 : 16); }
 
-template <int D, int NT>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) kv4_split_kernel(const __grid_constant__ Kv4Args a) {
+template <int D, int NT, int FO>
+__global__ void __launch_bounds__(32 * split_warps(NT), 1) kv4_split_kernel(const __grid_constant__ Kv4Args a) {
     using Ge = Kv4Geo<D>;
-    constexpr int NB = Ge::NB, WX = Ge::WX, QR = 4 * NT;
+    constexpr int QR = query_rows<NT, FO>();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ uint64_t s_bar[kWarps][kStages];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    if (lane == 0) {
-#pragma unroll
-        for (int i = 0; i < kStages; i++) mbar_init(&s_bar[warp][i], 1);
-        fence_barrier_init();
-    }
-    __syncwarp();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t worker = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
-    Range r = find_range<D>(a, worker, static_cast<int64_t>(gridDim.x) * kWarps, lane);
-    if (worker == 0 && lane == 0 && a.plan) a.plan[0] = r.chunk;
+    const int chunk = warp * gridDim.x + blockIdx.x;  // a call with few chunks spreads them over the SMs
+    Chunk w = find_chunk<D>(a, chunk, lane);
+    if (w.begin >= w.end) return;
+    const int64_t chunk_begin = w.begin;
     uint8_t* ring = smem + warp * Ge::WARP;
     float4* s_kd = reinterpret_cast<float4*>(ring + kStages * Ge::STAGE);
     uint4* s_vd = reinterpret_cast<uint4*>(ring + kStages * Ge::STAGE + Ge::DEC / 2);
-    const int64_t range_begin = r.begin;
-    uint32_t count = 0;  // tiles consumed from the ring so far
-    while (r.begin < r.end) {
-        const int seq = r.seq, kvh = r.head_group / a.q_groups, qg = r.head_group - kvh * a.q_groups, L = r.L;
+    const uint32_t ring_u32 = smem_u32(ring);
+    while (true) {  // the units of the chunk
+        const int seq = w.seq, kvh = w.head_group / a.q_groups, qg = w.head_group - kvh * a.q_groups, L = w.L;
         const int r0 = qg * QR, r_last = min(r0 + QR, a.q_rows) - 1;
-        const int ut = unit_tiles<D>(L), t0 = static_cast<int>(r.begin - r.first);
-        const int t1 = static_cast<int>(min(static_cast<int64_t>(ut), t0 + (r.end - r.begin)));
+        const int ut = unit_tiles<D>(L), t0 = static_cast<int>(w.begin - w.first);
+        const int t1 = static_cast<int>(min(static_cast<int64_t>(ut), t0 + (w.end - w.begin)));
         // rows that query row q sees: L - tokens + 1 + its token; the last one's bounds the rows worth reading
         const int min_lim = L - a.tokens + 1 + r0 / a.group;
         const int row_end = min(L, L - a.tokens + 1 + r_last / a.group);
         const int n = min(t1, row_end > 0 ? (row_end + Ge::TK - 1) / Ge::TK : 0) - t0;  // tiles with visible rows
-        if (lane == 0) {
-            for (int i = 0; i < min(kStages, n); i++)
-                load_tile<D>(a, seq, kvh, (t0 + i) * Ge::TK, row_end, ring + ((count + i) % kStages) * Ge::STAGE,
-                             &s_bar[warp][(count + i) % kStages]);
+        const TileCopy copy = tile_copy<D>(a, seq, kvh, lane);
+#pragma unroll
+        for (int i = 0; i < kStages - 1; i++) {
+            if (i < n) load_tile<D>(a, copy, seq, kvh, (t0 + i) * Ge::TK, row_end, ring_u32 + i * Ge::STAGE, lane);
+            cp_async_commit();
         }
-        uint32_t qb[NT][NB][4];
-        RowState<D, NT> s;
-        load_queries<D, NT>(a, seq, kvh, r0, L, qb, s, g, t);
-        for (int it = 0; it < n; it++, count++) {
-            const int stage = count % kStages, row0 = (t0 + it) * Ge::TK;
-            uint8_t* st = ring + stage * Ge::STAGE;
-            int gone = 0;
-            const AbortState ab{&gone, a.err, kWaitLimitNs};
-            if (!__all_sync(0xffffffffu, mbar_wait(&s_bar[warp][stage], (count / kStages) & 1, ab))) {
-                // given up (reported): none of this warp's copies may still be in flight when the CTA ends
-                for (int j = 0; j < min(kStages, n - it); j++) {
-                    int late = 0;
-                    mbar_wait(&s_bar[warp][(count + j) % kStages], ((count + j) / kStages) & 1, AbortState{&late, a.err, kWaitLimitNs});
-                }
-                return;
-            }
-            decode_headers<D>(st, s_kd, s_vd, row_end - row0, lane);
+        RowState<D, NT, FO> s;
+        load_queries<D, NT, FO>(a, seq, kvh, r0, L, s, g, t);
+        for (int it = 0, stage = 0; it < n; it++) {
+            cp_async_wait<kStages - 2>();
+            __syncwarp();  // the tile has landed for every lane, and every lane is done with the stage refilled below
+            const int free_stage = stage == 0 ? kStages - 1 : stage - 1;
+            if (it + kStages - 1 < n)
+                load_tile<D>(a, copy, seq, kvh, (t0 + it + kStages - 1) * Ge::TK, row_end, ring_u32 + free_stage * Ge::STAGE, lane);
+            cp_async_commit();
+            const uint8_t* st = ring + stage * Ge::STAGE;
+            decode_headers<D>(st, s_kd, s_vd, lane);
             __syncwarp();
-            compute_tile<D, NT>(st, s_kd, s_vd, row0, min_lim, qb, s, g, t);
-            __syncwarp();  // every lane is done with the stage and the decoded headers
-            if (lane == 0 && it + kStages < n)
-                load_tile<D>(a, seq, kvh, row0 + kStages * Ge::TK, row_end, st, &s_bar[warp][stage]);
+            compute_tile<D, NT, FO>(st, s_kd, s_vd, (t0 + it) * Ge::TK, min_lim, s, lane);
+            stage = stage + 1 == kStages ? 0 : stage + 1;
         }
-        // A unit that lies wholly in this worker's range is finished here; else its part goes to a record: slot 0 for the part
-        // that starts the range, slot 1 for one that starts within it.
+        __syncwarp();  // the next unit's copies go to stages that every lane has read
+        // A unit that lies wholly in this chunk is finished here, else its part goes to a record. Parts are numbered chunk +
+        // unit: along the row of tiles every next part has a higher number, and a unit's parts follow one another.
         const bool whole = t1 - t0 == ut;
-        if (t0 == 0 && lane == 0 && a.plan) a.plan[1 + (static_cast<int64_t>(seq) * a.n_kv_heads + kvh) * a.q_groups + qg] = r.first;
-        float* rec0 = a.partial + (worker * 2 + (r.begin > range_begin ? 1 : 0)) * QR * Ge::REC;
+        const int64_t unit = static_cast<int64_t>(seq) * a.n_kv_heads * a.q_groups + w.head_group;
+        if (t0 == 0 && lane == 0 && a.plan) {
+            const int64_t in_chunk = w.begin - chunk_begin;  // tiles of the chunk before the unit
+            a.plan[unit] = make_int2(chunk, static_cast<int>((in_chunk + ut - 1) / w.size) + 1);
+        }
+        float* rec0 = a.partial + (chunk + unit) * QR * Ge::REC;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             float l = s.l[nt];
 #pragma unroll
-            for (int o = 4; o <= 16; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            for (int o = 4 / FO; o <= 16; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+#pragma unroll
+            for (int o = 4 / FO; o < 4; o <<= 1)
+#pragma unroll
+                for (int c = 0; c < Ge::CPR; c++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s.o[nt][c][e] += __shfl_xor_sync(0xffffffffu, s.o[nt][c][e], o);
             const int row = 4 * nt + t, rr = r0 + row;
-            if (rr >= a.q_rows) continue;
+            if (t >= 4 / FO || rr >= a.q_rows) continue;
             const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-            for (int x = 0; x < WX; x++) {
-                const int ch = 32 * ((WX * g + x) % NB) + 8 * (g >> 1);
-                float (&o)[8] = s.o[nt][x];
+            for (int c = 0; c < Ge::CPR; c++) {
+                const int ch = Ge::v_channel(g, c);
+                float (&o)[4] = s.o[nt][c];
                 if (whole) {
-                    const int64_t at = seq * a.out_seq_stride + (rr / a.group) * a.out_token_stride +
-                                       static_cast<int64_t>(kvh * a.group + rr % a.group) * D + ch;
+                    const int64_t out = seq * a.out_seq_stride + (rr / a.group) * a.out_token_stride +
+                                        static_cast<int64_t>(kvh * a.group + rr % a.group) * D + ch;
 #pragma unroll
-                    for (int e = 0; e < 8; e++) o[e] = l == 0.f ? 0.f : o[e] * inv;
-                    if (a.out_f16) {
-                        *reinterpret_cast<uint4*>(static_cast<__half*>(a.out) + at) =
-                            make_uint4(pack_half2(o[0], o[1]), pack_half2(o[2], o[3]), pack_half2(o[4], o[5]), pack_half2(o[6], o[7]));
-                    } else {
-                        float4* p = reinterpret_cast<float4*>(static_cast<float*>(a.out) + at);
-                        p[0] = make_float4(o[0], o[1], o[2], o[3]);
-                        p[1] = make_float4(o[4], o[5], o[6], o[7]);
-                    }
+                    for (int e = 0; e < 4; e++) o[e] = l == 0.f ? 0.f : o[e] * inv;
+                    if (a.out_f16) *reinterpret_cast<uint2*>(static_cast<__half*>(a.out) + out) = make_uint2(pack_half2(o[0], o[1]), pack_half2(o[2], o[3]));
+                    else *reinterpret_cast<float4*>(static_cast<float*>(a.out) + out) = make_float4(o[0], o[1], o[2], o[3]);
                 } else {
-                    float4* p = reinterpret_cast<float4*>(rec0 + row * Ge::REC + ch);
-                    p[0] = make_float4(o[0], o[1], o[2], o[3]);
-                    p[1] = make_float4(o[4], o[5], o[6], o[7]);
+                    *reinterpret_cast<float4*>(rec0 + row * Ge::REC + ch) = make_float4(o[0], o[1], o[2], o[3]);
                 }
             }
             if (!whole && g == 0)
-                *reinterpret_cast<float2*>(rec0 + row * Ge::REC + D) =
-                    make_float2(s.m[nt] == -INFINITY ? -INFINITY : s.fs[nt] * s.m[nt], l);
+                *reinterpret_cast<float2*>(rec0 + row * Ge::REC + D) = make_float2(s.m[nt] == -INFINITY ? -INFINITY : s.fs[nt] * s.m[nt], l);
         }
-        r.begin += t1 - t0;
-        if (r.begin >= r.end) break;
-        r.first = r.begin;  // the next unit
-        if (++r.head_group == a.n_kv_heads * a.q_groups) {
-            r.head_group = 0;
-            r.seq++;
-            r.L = ctx_of(a, r.seq);
+        w.begin += t1 - t0;
+        if (w.begin >= w.end) return;
+        w.first = w.begin;  // the next unit
+        if (++w.head_group == a.n_kv_heads * a.q_groups) {
+            w.head_group = 0;
+            w.seq++;
+            w.L = ctx_of(a, w.seq);
         }
     }
 }
 
 // ------------------------------------------------------------------------------------------------ combine
 
-// One CTA per query row: its warps sum every fourth record of the row's unit, rescaled to the common maximum.
-template <int D, int NT>
-__global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const __grid_constant__ Kv4Args a) {
-    constexpr int EPL = D / 32, REC = Kv4Geo<D>::REC, QR = 4 * NT;
-    __shared__ float s_acc[kWarps][D];
-    __shared__ float s_ml[kWarps][2];
+constexpr int kCombineWarps = 4;
+constexpr int kCombineHeld = 4;  // records a warp has in flight
+
+// One CTA per query row: its warps take every fourth record of the row's unit, each with a running maximum.
+template <int D, int QR>
+__global__ void __launch_bounds__(32 * kCombineWarps) kv4_combine_kernel(const __grid_constant__ Kv4Args a) {
+    constexpr int EPL = D / 32, REC = Kv4Geo<D>::REC;
+    __shared__ float s_acc[kCombineWarps][D];
+    __shared__ float s_ml[kCombineWarps][2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rr = blockIdx.x % a.q_rows, kvh = (blockIdx.x / a.q_rows) % a.n_kv_heads, seq = blockIdx.x / (a.q_rows * a.n_kv_heads);
+    const int64_t unit = (static_cast<int64_t>(seq) * a.n_kv_heads + kvh) * a.q_groups + rr / QR;
     // Every CTA waits for the split grid, so that a later launch which sees this grid complete sees the split kernel's
     // writes too.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int rr = blockIdx.x % a.q_rows, kvh = (blockIdx.x / a.q_rows) % a.n_kv_heads, seq = blockIdx.x / (a.q_rows * a.n_kv_heads);
-    const int64_t chunk = a.plan[0], first = a.plan[1 + (static_cast<int64_t>(seq) * a.n_kv_heads + kvh) * a.q_groups + rr / QR];
-    const int tiles = unit_tiles<D>(ctx_of(a, seq));
-    const int64_t w0 = first / chunk, w1 = (first + tiles - 1) / chunk;
-    if (w0 == w1) return;  // written by the split kernel
-    const int n = static_cast<int>(w1 - w0) + 1;
-    const auto record = [&](int i) {  // part i: in the first worker's slot 1 unless the unit starts that worker's range
-        const int64_t w = w0 + i;
-        return a.partial + ((w * 2 + (i == 0 && first > w0 * chunk ? 1 : 0)) * QR + rr % QR) * REC;
-    };
-    float m = -INFINITY;
-    for (int i = warp + kWarps * lane; i < n; i += kWarps * 32) m = fmaxf(m, record(i)[D]);
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float acc[EPL], l = 0.f;
+    const int2 part = a.plan[unit];
+    if (part.y <= 1) return;  // written by the split kernel
+    const float* base = a.partial + ((part.x + unit) * QR + rr % QR) * REC;
+    float m = -INFINITY, l = 0.f, acc[EPL];
 #pragma unroll
     for (int e = 0; e < EPL; e++) acc[e] = 0.f;
-#pragma unroll 4
-    for (int i = warp; i < n; i += kWarps) {
-        const float* p = record(i);
-        const float2 ml = *reinterpret_cast<const float2*>(p + D);
-        const float f = m == -INFINITY ? 1.f : ex2_approx(ml.x - m);
-        l = fmaf(ml.y, f, l);
+    for (int i0 = warp; i0 < part.y; i0 += kCombineWarps * kCombineHeld) {
+        float2 ml[kCombineHeld];
+        float v[kCombineHeld][EPL];
 #pragma unroll
-        for (int e = 0; e < EPL; e++) acc[e] = fmaf(p[lane + 32 * e], f, acc[e]);
+        for (int k = 0; k < kCombineHeld; k++) {
+            const int i = i0 + k * kCombineWarps;
+            const float* p = base + static_cast<int64_t>(i) * QR * REC;
+            ml[k] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int e = 0; e < EPL; e++) v[k][e] = 0.f;
+            if (i < part.y) {
+                ml[k] = *reinterpret_cast<const float2*>(p + D);
+#pragma unroll
+                for (int e = 0; e < EPL; e++) v[k][e] = p[lane + 32 * e];
+            }
+        }
+        float top = m;
+#pragma unroll
+        for (int k = 0; k < kCombineHeld; k++) top = fmaxf(top, ml[k].x);
+        const float ref = top == -INFINITY ? 0.f : top;
+        const float alpha = ex2_approx(m - ref);
+        l *= alpha;
+#pragma unroll
+        for (int e = 0; e < EPL; e++) acc[e] *= alpha;
+#pragma unroll
+        for (int k = 0; k < kCombineHeld; k++) {
+            // a part whose maximum is -inf holds zeros, or NaN where its scores are NaN
+            const float f = ml[k].x == -INFINITY ? 1.f : ex2_approx(ml[k].x - ref);
+            l = fmaf(ml[k].y, f, l);
+#pragma unroll
+            for (int e = 0; e < EPL; e++) acc[e] = fmaf(v[k][e], f, acc[e]);
+        }
+        m = top;
     }
 #pragma unroll
     for (int e = 0; e < EPL; e++) s_acc[warp][lane + 32 * e] = acc[e];
@@ -647,12 +724,12 @@ __global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const __grid_cons
     __syncthreads();
     float M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWarps; w++) M = fmaxf(M, s_ml[w][0]);
-    for (int col = threadIdx.x; col < D; col += kThreads) {
+    for (int w = 0; w < kCombineWarps; w++) M = fmaxf(M, s_ml[w][0]);
+    for (int col = threadIdx.x; col < D; col += 32 * kCombineWarps) {
         float o = 0.f, sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; w++) {
-            const float f = M == -INFINITY ? 1.f : ex2_approx(s_ml[w][0] - M);
+        for (int w = 0; w < kCombineWarps; w++) {
+            const float f = s_ml[w][0] == -INFINITY ? 1.f : ex2_approx(s_ml[w][0] - M);
             o = fmaf(s_acc[w][col], f, o);
             sum = fmaf(s_ml[w][1], f, sum);
         }
@@ -748,28 +825,31 @@ __global__ void __launch_bounds__(32 * kGenWarps) kv4_general_kernel(const __gri
 
 int max_context(const alpaca_kv4_attn_desc& d) { return d.ctx_lens ? d.max_ctx_len : d.start_position + d.tokens; }
 
-// Query rows per worker (4 NT: the fewest that hold the call's rows per KV head, up to 16) and workers: one resident wave, or
-// one per tile where the call has fewer (by its bound).
+// Query rows per unit and chunks. One or two query rows fold the columns (FO = 4 / 2; a tile of head_dim 128 has two 16-row
+// groups, so at most 2); otherwise 4 NT rows, the fewest that hold the call's rows per KV head, up to 16. Chunks: one per warp of
+// the machine, or one per tile where the call has fewer (by its bound).
 constexpr int kSms = 148;
 struct SplitPlan {
-    int nt, q_rows, q_groups;
-    int64_t units, workers;
-    bool combine;  // some unit may be split between workers
+    int nt, fo, q_rows, q_groups, ctas, chunks;
+    int64_t units;
+    bool combine;  // some unit may be split between chunks
+    int rows_per_unit() const { return 4 * nt / fo; }
 };
 SplitPlan split_plan(const alpaca_kv4_attn_desc& d) {
     SplitPlan p;
     p.q_rows = d.tokens * (d.n_heads / d.n_kv_heads);
     p.nt = p.q_rows <= 4 ? 1 : (p.q_rows <= 8 ? 2 : 4);
-    p.q_groups = (p.q_rows + 4 * p.nt - 1) / (4 * p.nt);
+    p.fo = p.q_rows == 1 ? (d.head_dim == 64 ? 4 : 2) : (p.q_rows == 2 ? 2 : 1);
+    p.q_groups = (p.q_rows + p.rows_per_unit() - 1) / p.rows_per_unit();
     p.units = static_cast<int64_t>(d.n_seqs) * d.n_kv_heads * p.q_groups;
     const int tk = 4096 / d.head_dim, tiles = std::max(1, (max_context(d) + tk - 1) / tk);
-    p.workers = std::min<int64_t>(p.units * tiles, kSms * kWarps * ctas_per_sm(d.head_dim, p.nt));
-    p.workers = (p.workers + kWarps - 1) / kWarps * kWarps;
+    p.chunks = static_cast<int>(std::min<int64_t>(p.units * tiles, static_cast<int64_t>(kSms) * split_warps(p.nt)));
+    p.ctas = std::min(p.chunks, kSms);
     p.combine = tiles > 1;
     return p;
 }
 size_t round_up(size_t n, size_t m) { return (n + m - 1) / m * m; }
-size_t plan_bytes(const SplitPlan& p) { return p.combine ? round_up(sizeof(int64_t) * (1 + p.units), 256) : 0; }
+size_t plan_bytes(const SplitPlan& p) { return p.combine ? round_up(sizeof(int2) * p.units, 256) : 0; }
 
 cudaLaunchConfig_t pdl_config(dim3 grid, int threads, size_t smem, cudaStream_t s, cudaLaunchAttribute* attr) {
     cudaLaunchConfig_t cfg = {};
@@ -784,31 +864,30 @@ cudaLaunchConfig_t pdl_config(dim3 grid, int threads, size_t smem, cudaStream_t 
     return cfg;
 }
 
-template <int D, int NT>
-cudaError_t launch_split_nt(const Kv4Args& a, const SplitPlan& p, cudaStream_t s) {
-    constexpr size_t smem = kWarps * Kv4Geo<D>::WARP;
-    const auto fn = kv4_split_kernel<D, NT>;
+template <int D, int NT, int FO>
+cudaError_t launch_split_form(const Kv4Args& a, const SplitPlan& p, cudaStream_t s) {
+    constexpr size_t smem = split_warps(NT) * Kv4Geo<D>::WARP;
+    const auto fn = kv4_split_kernel<D, NT, FO>;
     cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          static_cast<int>(smem));
     if (e != cudaSuccess) return e;
-    e = cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributePreferredSharedMemoryCarveout,
-                             static_cast<int>(cudaSharedmemCarveoutMaxShared));
-    if (e != cudaSuccess) return e;
     cudaLaunchAttribute attr;
-    const cudaLaunchConfig_t cfg =
-        pdl_config(dim3(static_cast<unsigned>(p.workers / kWarps), 1, 1), kThreads, smem, s, &attr);
+    const cudaLaunchConfig_t cfg = pdl_config(dim3(p.ctas, 1, 1), 32 * split_warps(NT), smem, s, &attr);
     e = cudaLaunchKernelEx(&cfg, fn, a);
     if (e != cudaSuccess || !p.combine) return e;
     const unsigned rows = static_cast<unsigned>(a.n_seqs) * a.n_kv_heads * a.q_rows;
-    const cudaLaunchConfig_t ccfg = pdl_config(dim3(rows, 1, 1), kThreads, 0, s, &attr);
-    return cudaLaunchKernelEx(&ccfg, kv4_combine_kernel<D, NT>, a);
+    const cudaLaunchConfig_t ccfg = pdl_config(dim3(rows, 1, 1), 32 * kCombineWarps, 0, s, &attr);
+    return cudaLaunchKernelEx(&ccfg, kv4_combine_kernel<D, query_rows<NT, FO>()>, a);
 }
 
 template <int D>
 cudaError_t launch_split(const Kv4Args& a, const SplitPlan& p, cudaStream_t s) {
-    return p.nt == 1   ? launch_split_nt<D, 1>(a, p, s)
-           : p.nt == 2 ? launch_split_nt<D, 2>(a, p, s)
-                       : launch_split_nt<D, 4>(a, p, s);
+    if constexpr (D == 64)
+        if (p.fo == 4) return launch_split_form<D, 1, 4>(a, p, s);
+    return p.fo == 2    ? launch_split_form<D, 1, 2>(a, p, s)
+           : p.nt == 1  ? launch_split_form<D, 1, 1>(a, p, s)
+           : p.nt == 2  ? launch_split_form<D, 2, 1>(a, p, s)
+                        : launch_split_form<D, 4, 1>(a, p, s);
 }
 
 // The prompt-chunk form: the visible rows as f16 in the workspace ([seq][row][kv_head][d], exact), then the tensor-core
@@ -858,7 +937,7 @@ ChunkPlan chunk_plan(const alpaca_kv4_attn_desc& d, void* ws) {
 size_t kv4_workspace_bytes(const alpaca_kv4_attn_desc& d, alpaca_attn_kernel kind) {
     if (kind == ALPACA_ATTN_DECODE_SPLIT) {
         const SplitPlan p = split_plan(d);
-        return p.combine ? plan_bytes(p) + sizeof(float) * p.workers * 2 * 4 * p.nt * (d.head_dim + 4) : 0;
+        return p.combine ? plan_bytes(p) + sizeof(float) * (p.chunks + p.units) * p.rows_per_unit() * (d.head_dim + 4) : 0;
     }
     if (kind == ALPACA_ATTN_PREFILL_TC) {
         const ChunkPlan p = chunk_plan(d, nullptr);
@@ -914,13 +993,15 @@ cudaError_t launch_kv4_attention(const alpaca_kv4_attn_desc& d, alpaca_attn_kern
         const SplitPlan p = split_plan(d);
         a.q_rows = p.q_rows;
         a.q_groups = p.q_groups;
+        a.chunks = p.chunks;
         if (p.combine) {
-            a.plan = static_cast<int64_t*>(ws);
+            a.plan = static_cast<int2*>(ws);
             a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + plan_bytes(p));
         }
         return d.head_dim == 128 ? launch_split<128>(a, p, s) : launch_split<64>(a, p, s);
     }
     a.q_rows = a.q_groups = 0;
+    a.chunks = 0;
     const int64_t rows = static_cast<int64_t>(d.n_seqs) * d.tokens * d.n_heads;
     cudaLaunchAttribute attr;
     const cudaLaunchConfig_t cfg =
