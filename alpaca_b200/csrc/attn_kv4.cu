@@ -158,11 +158,43 @@ __device__ __forceinline__ TileCopy tile_copy(const Kv4Args& a, int64_t unit, in
     return c;
 }
 
-// Copies rows [row0, min(row0 + TK, row_end)) of one KV head into a stage. The rows past them, and rows of a table entry
-// outside the pool, read as zero codes with step 0. The caller commits the group.
+// Where a warp's tiles lie in a paged cache whose blocks hold whole tiles: block `b` of the sequence, row `r` of it, and 32
+// entries of its table from `base` on, one per lane.
+struct Pages {
+    int b, r, base, entry;
+};
 template <int D>
-__device__ __forceinline__ void load_tile(const Kv4Args& a, const TileCopy& head, int seq, int kvh, int row0, int row_end, uint32_t stage,
-                                          int lane) {
+__device__ __forceinline__ Pages first_page(const Kv4Args& a, int row0) {
+    Pages p;
+    p.b = a.c.block_table ? row0 / a.c.rows : 0;
+    p.r = row0 - p.b * a.c.rows;
+    p.base = -64;
+    p.entry = -1;
+    return p;
+}
+// Block of the tile that the pages stand at, which then move on by a tile; -1 (reported) when the entry is outside the pool.
+template <int D>
+__device__ __forceinline__ int next_page(const Kv4Args& a, Pages& p, int seq, int lane) {
+    if (p.b >= p.base + 32) {
+        p.base = p.b;
+        p.entry = p.b + lane < a.c.max_blocks ? a.c.block_table[static_cast<int64_t>(seq) * a.c.max_blocks + p.b + lane] : -1;
+    }
+    const int blk = __shfl_sync(0xffffffffu, p.entry, p.b - p.base);
+    p.r += Kv4Geo<D>::TK;
+    if (p.r >= a.c.rows) {
+        p.r = 0;
+        p.b++;
+    }
+    if (blk >= 0 && blk < a.c.pool_blocks) return blk;
+    atomicOr(a.err, kDevErrBadIndex);
+    return -1;
+}
+
+// Copies rows [row0, min(row0 + TK, row_end)) of one KV head into a stage. The rows past them, and rows of a table entry
+// outside the pool, read as zero codes with step 0. Calls for a unit go from tile to tile. The caller commits the group.
+template <int D>
+__device__ __forceinline__ void load_tile(const Kv4Args& a, const TileCopy& head, Pages& pages, int seq, int kvh, int row0, int row_end,
+                                          uint32_t stage, int lane) {
     using Ge = Kv4Geo<D>;
     const int n = row_end - row0;
     TileCopy c = head;
@@ -170,8 +202,13 @@ __device__ __forceinline__ void load_tile(const Kv4Args& a, const TileCopy& head
     int r = row0;
     bool whole = n >= Ge::TK;  // a full tile of one unit: one run of bytes per plane
     if (a.c.block_table) {
-        whole = whole && a.c.rows % Ge::TK == 0 && kv4_locate(a.c, seq, row0, a.err, unit, r);
-        if (whole) c = tile_copy<D>(a, unit, kvh, lane);
+        whole = whole && a.c.rows % Ge::TK == 0;
+        if (whole) {
+            r = pages.r;
+            unit = next_page<D>(a, pages, seq, lane);
+            whole = unit >= 0;
+            if (whole) c = tile_copy<D>(a, unit, kvh, lane);
+        }
     }
     if (whole) {
         const uint8_t* k = c.k + static_cast<int64_t>(r) * Ge::CROW;
@@ -409,14 +446,24 @@ template <int D>
 __device__ __forceinline__ int unit_tiles(int L) {
     return max(1, (L + Kv4Geo<D>::TK - 1) / Kv4Geo<D>::TK);
 }
+constexpr int kUnitCost = 2;  // what a unit costs besides its tiles (queries, first copies), in tiles
 
-// The work of a call is its units' tiles in one row, sequence by sequence, cut into equal chunks, one per warp: all warps of
-// the one resident wave then have the same number of tiles, whatever the contexts are.
+// a / b for a >= 0, b > 0, by 32-bit division where the operands allow it.
+__device__ __forceinline__ int64_t div_pos(int64_t a, int64_t b) {
+    return (a | b) >> 32 ? a / b : static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b));
+}
+
+// The work of a call is its units in one row, sequence by sequence, each kUnitCost places and then one place per tile. The row
+// is cut into equal chunks, one per warp: all warps of the one resident wave then have the same work, whatever the contexts are.
 struct Chunk {
-    int64_t begin, end, size;  // tiles; `size` of every chunk but the last
-    int64_t first;             // first tile of the unit that `begin` lies in
+    int64_t begin, end, size;  // places; `size` of every chunk but the last
+    int64_t first;             // first place of the unit that `begin` lies in
     int seq, head_group, L;    // that unit: sequence, kv_head * q_groups + query group, the sequence's context
 };
+template <int D>
+__device__ __forceinline__ int unit_places(int L) {
+    return kUnitCost + unit_tiles<D>(L);
+}
 
 template <int D>
 __device__ __forceinline__ Chunk find_chunk(const Kv4Args& a, int64_t index, int lane) {
@@ -429,34 +476,34 @@ __device__ __forceinline__ Chunk find_chunk(const Kv4Args& a, int64_t index, int
 #pragma unroll
         for (int i = 0; i < HELD; i++) held[i] = lane + 32 * i < a.n_seqs ? ctx_of(a, lane + 32 * i) : 0;
 #pragma unroll
-        for (int i = 0; i < HELD; i++) total += lane + 32 * i < a.n_seqs ? unit_tiles<D>(held[i]) : 0;
-        for (int s = lane + 32 * HELD; s < a.n_seqs; s += 32) total += unit_tiles<D>(ctx_of(a, s));
+        for (int i = 0; i < HELD; i++) total += lane + 32 * i < a.n_seqs ? unit_places<D>(held[i]) : 0;
+        for (int s = lane + 32 * HELD; s < a.n_seqs; s += 32) total += unit_places<D>(ctx_of(a, s));
         // a lane's sum is below 2^36: two 32-bit sums hold the warp's
         const unsigned lo = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(total & 0xFFFFF));
         const unsigned hi = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(total >> 20));
         total = (static_cast<int64_t>(hi) << 20) + lo;
     } else {
-        total = static_cast<int64_t>(a.n_seqs) * unit_tiles<D>(a.uniform_len);
+        total = static_cast<int64_t>(a.n_seqs) * unit_places<D>(a.uniform_len);
     }
     total *= hg;
-    c.size = (total + a.chunks - 1) / a.chunks;
+    c.size = div_pos(total + a.chunks - 1, a.chunks);
     c.begin = index * c.size;
     c.end = min(c.begin + c.size, total);
     if (c.begin >= c.end) return c;
     if (!a.ctx_lens) {
-        const int t = unit_tiles<D>(a.uniform_len);
-        const int64_t unit = c.begin / t;
+        const int t = unit_places<D>(a.uniform_len);
+        const int64_t unit = div_pos(c.begin, t);
         c.first = unit * t;
-        c.seq = static_cast<int>(unit / hg);
+        c.seq = static_cast<int>(div_pos(unit, hg));
         c.head_group = static_cast<int>(unit - c.seq * hg);
         c.L = a.uniform_len;
         return c;
     }
-    int64_t before = 0;  // tiles before the block of 32 sequences
+    int64_t before = 0;  // places before the block of 32 sequences
     for (int s0 = 0;; s0 += 32) {
         const int s = s0 + lane;
         const int L = s0 == 0 ? held[0] : (s0 == 32 ? held[1] : (s < a.n_seqs ? ctx_of(a, s) : 0));
-        const int mine = s < a.n_seqs ? unit_tiles<D>(L) : 0;  // at most 2^25: a block's sum fits 32 bits
+        const int mine = s < a.n_seqs ? unit_places<D>(L) : 0;  // at most 2^25 + 1: a block's sum fits 32 bits
         int incl = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -469,8 +516,8 @@ __device__ __forceinline__ Chunk find_chunk(const Kv4Args& a, int64_t index, int
             c.seq = s0 + src;
             c.L = __shfl_sync(0xffffffffu, L, src);
             const int64_t start = before + __shfl_sync(0xffffffffu, incl - mine, src) * hg;
-            const int t = unit_tiles<D>(c.L);
-            c.head_group = static_cast<int>((c.begin - start) / t);
+            const int t = unit_places<D>(c.L);
+            c.head_group = static_cast<int>(div_pos(c.begin - start, t));
             c.first = start + static_cast<int64_t>(c.head_group) * t;
             return c;
         }
@@ -577,16 +624,19 @@ __global__ void __launch_bounds__(32 * split_warps(NT), 1) kv4_split_kernel(cons
     while (true) {  // the units of the chunk
         const int seq = w.seq, kvh = w.head_group / a.q_groups, qg = w.head_group - kvh * a.q_groups, L = w.L;
         const int r0 = qg * QR, r_last = min(r0 + QR, a.q_rows) - 1;
-        const int ut = unit_tiles<D>(L), t0 = static_cast<int>(w.begin - w.first);
-        const int t1 = static_cast<int>(min(static_cast<int64_t>(ut), t0 + (w.end - w.begin)));
+        const int64_t tile0 = w.first + kUnitCost;  // place of the unit's first tile
+        const int ut = unit_tiles<D>(L), t0 = static_cast<int>(max(w.begin - tile0, static_cast<int64_t>(0)));
+        const int t1 = static_cast<int>(min(static_cast<int64_t>(ut), w.end - tile0));
+        if (t1 <= t0) return;  // the chunk ends in the places before the unit's first tile
         // rows that query row q sees: L - tokens + 1 + its token; the last one's bounds the rows worth reading
         const int min_lim = L - a.tokens + 1 + r0 / a.group;
         const int row_end = min(L, L - a.tokens + 1 + r_last / a.group);
         const int n = min(t1, row_end > 0 ? (row_end + Ge::TK - 1) / Ge::TK : 0) - t0;  // tiles with visible rows
-        const TileCopy copy = tile_copy<D>(a, seq, kvh, lane);
+        const TileCopy copy = tile_copy<D>(a, a.c.block_table ? 0 : seq, kvh, lane);
+        Pages pages = first_page<D>(a, t0 * Ge::TK);
 #pragma unroll
         for (int i = 0; i < kStages - 1; i++) {
-            if (i < n) load_tile<D>(a, copy, seq, kvh, (t0 + i) * Ge::TK, row_end, ring_u32 + i * Ge::STAGE, lane);
+            if (i < n) load_tile<D>(a, copy, pages, seq, kvh, (t0 + i) * Ge::TK, row_end, ring_u32 + i * Ge::STAGE, lane);
             cp_async_commit();
         }
         RowState<D, NT, FO> s;
@@ -596,7 +646,7 @@ __global__ void __launch_bounds__(32 * split_warps(NT), 1) kv4_split_kernel(cons
             __syncwarp();  // the tile has landed for every lane, and every lane is done with the stage refilled below
             const int free_stage = stage == 0 ? kStages - 1 : stage - 1;
             if (it + kStages - 1 < n)
-                load_tile<D>(a, copy, seq, kvh, (t0 + it + kStages - 1) * Ge::TK, row_end, ring_u32 + free_stage * Ge::STAGE, lane);
+                load_tile<D>(a, copy, pages, seq, kvh, (t0 + it + kStages - 1) * Ge::TK, row_end, ring_u32 + free_stage * Ge::STAGE, lane);
             cp_async_commit();
             const uint8_t* st = ring + stage * Ge::STAGE;
             decode_headers<D>(st, s_kd, s_vd, lane);
@@ -610,8 +660,7 @@ __global__ void __launch_bounds__(32 * split_warps(NT), 1) kv4_split_kernel(cons
         const bool whole = t1 - t0 == ut;
         const int64_t unit = static_cast<int64_t>(seq) * a.n_kv_heads * a.q_groups + w.head_group;
         if (t0 == 0 && lane == 0 && a.plan) {
-            const int64_t in_chunk = w.begin - chunk_begin;  // tiles of the chunk before the unit
-            a.plan[unit] = make_int2(chunk, static_cast<int>((in_chunk + ut - 1) / w.size) + 1);
+            a.plan[unit] = make_int2(chunk, static_cast<int>(div_pos(tile0 - chunk_begin + ut - 1, w.size)) + 1);
         }
         float* rec0 = a.partial + (chunk + unit) * QR * Ge::REC;
 #pragma unroll
@@ -646,9 +695,8 @@ __global__ void __launch_bounds__(32 * split_warps(NT), 1) kv4_split_kernel(cons
             if (!whole && g == 0)
                 *reinterpret_cast<float2*>(rec0 + row * Ge::REC + D) = make_float2(s.m[nt] == -INFINITY ? -INFINITY : s.fs[nt] * s.m[nt], l);
         }
-        w.begin += t1 - t0;
+        w.first = w.begin = tile0 + ut;  // the next unit
         if (w.begin >= w.end) return;
-        w.first = w.begin;  // the next unit
         if (++w.head_group == a.n_kv_heads * a.q_groups) {
             w.head_group = 0;
             w.seq++;
@@ -827,7 +875,7 @@ int max_context(const alpaca_kv4_attn_desc& d) { return d.ctx_lens ? d.max_ctx_l
 
 // Query rows per unit and chunks. One or two query rows fold the columns (FO = 4 / 2; a tile of head_dim 128 has two 16-row
 // groups, so at most 2); otherwise 4 NT rows, the fewest that hold the call's rows per KV head, up to 16. Chunks: one per warp of
-// the machine, or one per tile where the call has fewer (by its bound).
+// the machine, or one per place where the call has fewer (by its bound).
 constexpr int kSms = 148;
 struct SplitPlan {
     int nt, fo, q_rows, q_groups, ctas, chunks;
@@ -843,7 +891,7 @@ SplitPlan split_plan(const alpaca_kv4_attn_desc& d) {
     p.q_groups = (p.q_rows + p.rows_per_unit() - 1) / p.rows_per_unit();
     p.units = static_cast<int64_t>(d.n_seqs) * d.n_kv_heads * p.q_groups;
     const int tk = 4096 / d.head_dim, tiles = std::max(1, (max_context(d) + tk - 1) / tk);
-    p.chunks = static_cast<int>(std::min<int64_t>(p.units * tiles, static_cast<int64_t>(kSms) * split_warps(p.nt)));
+    p.chunks = static_cast<int>(std::min<int64_t>(p.units * (kUnitCost + tiles), static_cast<int64_t>(kSms) * split_warps(p.nt)));
     p.ctas = std::min(p.chunks, kSms);
     p.combine = tiles > 1;
     return p;
