@@ -44,6 +44,7 @@ struct Kv4Args {
     int2* plan;      // [unit]: the first chunk that holds tiles of it, and how many do
     float* partial;  // [chunk + unit][query row of the group][d + 4]: accumulators, m (log2 units), l
     int chunks;
+    int cta_units;   // one CTA per unit: its warps share the unit's tiles and meet in shared memory (no records)
     float scale;
     unsigned* err;
 };
@@ -172,29 +173,27 @@ __device__ __forceinline__ Pages first_page(const Kv4Args& a, int row0) {
     p.entry = -1;
     return p;
 }
-// Block of the tile that the pages stand at, which then move on by a tile; -1 (reported) when the entry is outside the pool.
+// Block of the tile that the pages stand at, which then move on by `step` tiles; -1 (reported) when the entry is outside the
+// pool.
 template <int D>
-__device__ __forceinline__ int next_page(const Kv4Args& a, Pages& p, int seq, int lane) {
+__device__ __forceinline__ int next_page(const Kv4Args& a, Pages& p, int seq, int step, int lane) {
     if (p.b >= p.base + 32) {
         p.base = p.b;
         p.entry = p.b + lane < a.c.max_blocks ? a.c.block_table[static_cast<int64_t>(seq) * a.c.max_blocks + p.b + lane] : -1;
     }
     const int blk = __shfl_sync(0xffffffffu, p.entry, p.b - p.base);
-    p.r += Kv4Geo<D>::TK;
-    if (p.r >= a.c.rows) {
-        p.r = 0;
-        p.b++;
-    }
+    for (p.r += step * Kv4Geo<D>::TK; p.r >= a.c.rows; p.r -= a.c.rows) p.b++;
     if (blk >= 0 && blk < a.c.pool_blocks) return blk;
     atomicOr(a.err, kDevErrBadIndex);
     return -1;
 }
 
 // Copies rows [row0, min(row0 + TK, row_end)) of one KV head into a stage. The rows past them, and rows of a table entry
-// outside the pool, read as zero codes with step 0. Calls for a unit go from tile to tile. The caller commits the group.
+// outside the pool, read as zero codes with step 0. Calls for a unit go from tile to tile, `step` at a time. The caller commits
+// the group.
 template <int D>
 __device__ __forceinline__ void load_tile(const Kv4Args& a, const TileCopy& head, Pages& pages, int seq, int kvh, int row0, int row_end,
-                                          uint32_t stage, int lane) {
+                                          int step, uint32_t stage, int lane) {
     using Ge = Kv4Geo<D>;
     const int n = row_end - row0;
     TileCopy c = head;
@@ -205,7 +204,7 @@ __device__ __forceinline__ void load_tile(const Kv4Args& a, const TileCopy& head
         whole = whole && a.c.rows % Ge::TK == 0;
         if (whole) {
             r = pages.r;
-            unit = next_page<D>(a, pages, seq, lane);
+            unit = next_page<D>(a, pages, seq, step, lane);
             whole = unit >= 0;
             if (whole) c = tile_copy<D>(a, unit, kvh, lane);
         }
@@ -613,30 +612,42 @@ __global__ void __launch_bounds__(32 * split_warps(NT), 1) kv4_split_kernel(cons
     extern __shared__ __align__(16) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int chunk = warp * gridDim.x + blockIdx.x;  // a call with few chunks spreads them over the SMs
-    Chunk w = find_chunk<D>(a, chunk, lane);
-    if (w.begin >= w.end) return;
-    const int64_t chunk_begin = w.begin;
     uint8_t* ring = smem + warp * Ge::WARP;
     float4* s_kd = reinterpret_cast<float4*>(ring + kStages * Ge::STAGE);
     uint4* s_vd = reinterpret_cast<uint4*>(ring + kStages * Ge::STAGE + Ge::DEC / 2);
     const uint32_t ring_u32 = smem_u32(ring);
+    const int chunk = warp * gridDim.x + blockIdx.x;  // a call with few chunks spreads them over the SMs
+    Chunk w;
+    if (a.cta_units) {
+        const int hg = a.n_kv_heads * a.q_groups;
+        w.seq = blockIdx.x / hg;
+        w.head_group = blockIdx.x - w.seq * hg;
+        w.L = ctx_of(a, w.seq);
+        w.begin = w.end = w.size = w.first = 0;
+    } else {
+        w = find_chunk<D>(a, chunk, lane);
+        if (w.begin >= w.end) return;
+    }
+    const int64_t chunk_begin = w.begin;
+    const int step = a.cta_units ? blockDim.x / 32 : 1;
     while (true) {  // the units of the chunk
         const int seq = w.seq, kvh = w.head_group / a.q_groups, qg = w.head_group - kvh * a.q_groups, L = w.L;
         const int r0 = qg * QR, r_last = min(r0 + QR, a.q_rows) - 1;
         const int64_t tile0 = w.first + kUnitCost;  // place of the unit's first tile
-        const int ut = unit_tiles<D>(L), t0 = static_cast<int>(max(w.begin - tile0, static_cast<int64_t>(0)));
-        const int t1 = static_cast<int>(min(static_cast<int64_t>(ut), w.end - tile0));
-        if (t1 <= t0) return;  // the chunk ends in the places before the unit's first tile
+        const int ut = unit_tiles<D>(L);
+        const int t0 = a.cta_units ? warp : static_cast<int>(max(w.begin - tile0, static_cast<int64_t>(0)));
+        const int t1 = a.cta_units ? ut : static_cast<int>(min(static_cast<int64_t>(ut), w.end - tile0));
+        if (!a.cta_units && t1 <= t0) return;  // the chunk ends in the places before the unit's first tile
         // rows that query row q sees: L - tokens + 1 + its token; the last one's bounds the rows worth reading
         const int min_lim = L - a.tokens + 1 + r0 / a.group;
         const int row_end = min(L, L - a.tokens + 1 + r_last / a.group);
-        const int n = min(t1, row_end > 0 ? (row_end + Ge::TK - 1) / Ge::TK : 0) - t0;  // tiles with visible rows
+        const int visible = min(t1, row_end > 0 ? (row_end + Ge::TK - 1) / Ge::TK : 0);
+        const int n = (max(visible - t0, 0) + step - 1) / step;  // tiles of this warp: t0, t0 + step, ..
         const TileCopy copy = tile_copy<D>(a, a.c.block_table ? 0 : seq, kvh, lane);
         Pages pages = first_page<D>(a, t0 * Ge::TK);
 #pragma unroll
         for (int i = 0; i < kStages - 1; i++) {
-            if (i < n) load_tile<D>(a, copy, pages, seq, kvh, (t0 + i) * Ge::TK, row_end, ring_u32 + i * Ge::STAGE, lane);
+            if (i < n) load_tile<D>(a, copy, pages, seq, kvh, (t0 + i * step) * Ge::TK, row_end, step, ring_u32 + i * Ge::STAGE, lane);
             cp_async_commit();
         }
         RowState<D, NT, FO> s;
@@ -646,23 +657,27 @@ __global__ void __launch_bounds__(32 * split_warps(NT), 1) kv4_split_kernel(cons
             __syncwarp();  // the tile has landed for every lane, and every lane is done with the stage refilled below
             const int free_stage = stage == 0 ? kStages - 1 : stage - 1;
             if (it + kStages - 1 < n)
-                load_tile<D>(a, copy, pages, seq, kvh, (t0 + it + kStages - 1) * Ge::TK, row_end, ring_u32 + free_stage * Ge::STAGE, lane);
+                load_tile<D>(a, copy, pages, seq, kvh, (t0 + (it + kStages - 1) * step) * Ge::TK, row_end, step,
+                             ring_u32 + free_stage * Ge::STAGE, lane);
             cp_async_commit();
             const uint8_t* st = ring + stage * Ge::STAGE;
             decode_headers<D>(st, s_kd, s_vd, lane);
             __syncwarp();
-            compute_tile<D, NT, FO>(st, s_kd, s_vd, (t0 + it) * Ge::TK, min_lim, s, lane);
+            compute_tile<D, NT, FO>(st, s_kd, s_vd, (t0 + it * step) * Ge::TK, min_lim, s, lane);
             stage = stage + 1 == kStages ? 0 : stage + 1;
         }
-        __syncwarp();  // the next unit's copies go to stages that every lane has read
         // A unit that lies wholly in this chunk is finished here, else its part goes to a record. Parts are numbered chunk +
-        // unit: along the row of tiles every next part has a higher number, and a unit's parts follow one another.
-        const bool whole = t1 - t0 == ut;
+        // unit: along the row of places every next part has a higher number, and a unit's parts follow one another. With one CTA
+        // per unit the parts are its warps', in shared memory over the rings.
+        const bool whole = !a.cta_units && t1 - t0 == ut;
         const int64_t unit = static_cast<int64_t>(seq) * a.n_kv_heads * a.q_groups + w.head_group;
-        if (t0 == 0 && lane == 0 && a.plan) {
+        if (!a.cta_units && t0 == 0 && lane == 0 && a.plan) {
             a.plan[unit] = make_int2(chunk, static_cast<int>(div_pos(tile0 - chunk_begin + ut - 1, w.size)) + 1);
         }
-        float* rec0 = a.partial + (chunk + unit) * QR * Ge::REC;
+        float* rec0 = a.cta_units ? reinterpret_cast<float*>(smem) + warp * QR * Ge::REC : a.partial + (chunk + unit) * QR * Ge::REC;
+        static_assert(sizeof(float) * QR * Ge::REC <= Ge::WARP, "a warp's record must fit its ring");
+        if (a.cta_units) __syncthreads();  // every warp is done with its ring
+        else __syncwarp();                 // the next unit's copies go to stages that every lane has read
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             float l = s.l[nt];
@@ -695,6 +710,26 @@ __global__ void __launch_bounds__(32 * split_warps(NT), 1) kv4_split_kernel(cons
             if (!whole && g == 0)
                 *reinterpret_cast<float2*>(rec0 + row * Ge::REC + D) = make_float2(s.m[nt] == -INFINITY ? -INFINITY : s.fs[nt] * s.m[nt], l);
         }
+        if (a.cta_units) {
+            __syncthreads();
+            const int warps = min(step, max(row_end > 0 ? (row_end + Ge::TK - 1) / Ge::TK : 0, 1));  // those with tiles
+            for (int i = threadIdx.x; i < QR * D; i += blockDim.x) {
+                const int row = i / D, col = i - row * D, rr = r0 + row;
+                if (rr >= a.q_rows) break;
+                const float* rec = reinterpret_cast<const float*>(smem) + row * Ge::REC;
+                float M = -INFINITY;
+                for (int k = 0; k < warps; k++) M = fmaxf(M, rec[k * QR * Ge::REC + D]);
+                float o = 0.f, l = 0.f;
+                for (int k = 0; k < warps; k++) {
+                    const float* p = rec + k * QR * Ge::REC;
+                    const float f = p[D] == -INFINITY ? 1.f : ex2_approx(p[D] - M);  // without a maximum: zeros, or NaN
+                    l = fmaf(p[D + 1], f, l);
+                    o = fmaf(p[col], f, o);
+                }
+                store_out(a, seq, rr / a.group, kvh * a.group + rr % a.group, D, col, l == 0.f ? 0.f : o / l);
+            }
+            return;
+        }
         w.first = w.begin = tile0 + ut;  // the next unit
         if (w.begin >= w.end) return;
         if (++w.head_group == a.n_kv_heads * a.q_groups) {
@@ -707,16 +742,16 @@ __global__ void __launch_bounds__(32 * split_warps(NT), 1) kv4_split_kernel(cons
 
 // ------------------------------------------------------------------------------------------------ combine
 
-constexpr int kCombineWarps = 4;
-constexpr int kCombineHeld = 4;  // records a warp has in flight
+constexpr int kCombineWarps = 16;  // at most
+constexpr int kCombineHeld = 4;    // records a warp has in flight
 
-// One CTA per query row: its warps take every fourth record of the row's unit, each with a running maximum.
+// One CTA per query row: its warps share the records of the row's unit, each with a running maximum.
 template <int D, int QR>
 __global__ void __launch_bounds__(32 * kCombineWarps) kv4_combine_kernel(const __grid_constant__ Kv4Args a) {
     constexpr int EPL = D / 32, REC = Kv4Geo<D>::REC;
     __shared__ float s_acc[kCombineWarps][D];
     __shared__ float s_ml[kCombineWarps][2];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x / 32;
     const int rr = blockIdx.x % a.q_rows, kvh = (blockIdx.x / a.q_rows) % a.n_kv_heads, seq = blockIdx.x / (a.q_rows * a.n_kv_heads);
     const int64_t unit = (static_cast<int64_t>(seq) * a.n_kv_heads + kvh) * a.q_groups + rr / QR;
     // Every CTA waits for the split grid, so that a later launch which sees this grid complete sees the split kernel's
@@ -725,16 +760,20 @@ __global__ void __launch_bounds__(32 * kCombineWarps) kv4_combine_kernel(const _
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int2 part = a.plan[unit];
     if (part.y <= 1) return;  // written by the split kernel
+    if (part.x < 0 || part.y > a.chunks - part.x) {  // not this call's plan: the workspace was written to meanwhile
+        atomicOr(a.err, kDevErrBadIndex);
+        return;
+    }
     const float* base = a.partial + ((part.x + unit) * QR + rr % QR) * REC;
     float m = -INFINITY, l = 0.f, acc[EPL];
 #pragma unroll
     for (int e = 0; e < EPL; e++) acc[e] = 0.f;
-    for (int i0 = warp; i0 < part.y; i0 += kCombineWarps * kCombineHeld) {
+    for (int i0 = warp; i0 < part.y; i0 += warps * kCombineHeld) {
         float2 ml[kCombineHeld];
         float v[kCombineHeld][EPL];
 #pragma unroll
         for (int k = 0; k < kCombineHeld; k++) {
-            const int i = i0 + k * kCombineWarps;
+            const int i = i0 + k * warps;
             const float* p = base + static_cast<int64_t>(i) * QR * REC;
             ml[k] = make_float2(-INFINITY, 0.f);
 #pragma unroll
@@ -771,12 +810,10 @@ __global__ void __launch_bounds__(32 * kCombineWarps) kv4_combine_kernel(const _
     }
     __syncthreads();
     float M = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kCombineWarps; w++) M = fmaxf(M, s_ml[w][0]);
-    for (int col = threadIdx.x; col < D; col += 32 * kCombineWarps) {
+    for (int w = 0; w < warps; w++) M = fmaxf(M, s_ml[w][0]);
+    for (int col = threadIdx.x; col < D; col += blockDim.x) {
         float o = 0.f, sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < kCombineWarps; w++) {
+        for (int w = 0; w < warps; w++) {
             const float f = s_ml[w][0] == -INFINITY ? 1.f : ex2_approx(s_ml[w][0] - M);
             o = fmaf(s_acc[w][col], f, o);
             sum = fmaf(s_ml[w][1], f, sum);
@@ -878,9 +915,10 @@ int max_context(const alpaca_kv4_attn_desc& d) { return d.ctx_lens ? d.max_ctx_l
 // the machine, or one per place where the call has fewer (by its bound).
 constexpr int kSms = 148;
 struct SplitPlan {
-    int nt, fo, q_rows, q_groups, ctas, chunks;
+    int nt, fo, q_rows, q_groups, ctas, warps, chunks;
     int64_t units;
-    bool combine;  // some unit may be split between chunks
+    bool cta_units;  // one CTA per unit, no records
+    bool combine;    // some unit may be split between chunks
     int rows_per_unit() const { return 4 * nt / fo; }
 };
 SplitPlan split_plan(const alpaca_kv4_attn_desc& d) {
@@ -892,8 +930,15 @@ SplitPlan split_plan(const alpaca_kv4_attn_desc& d) {
     p.units = static_cast<int64_t>(d.n_seqs) * d.n_kv_heads * p.q_groups;
     const int tk = 4096 / d.head_dim, tiles = std::max(1, (max_context(d) + tk - 1) / tk);
     p.chunks = static_cast<int>(std::min<int64_t>(p.units * (kUnitCost + tiles), static_cast<int64_t>(kSms) * split_warps(p.nt)));
-    p.ctas = std::min(p.chunks, kSms);
-    p.combine = tiles > 1;
+    // Few units of short contexts: one CTA per unit, one launch. With one tile a warp that wins always (9/3 heads, 517 rows:
+    // 4.8 us against 5.6); with more, only where the units fill the machine: two from 32 units on (48 units of 2000 rows: 8.2
+    // against 9.3; 12 units: 8.2 against 7.7), four from 96 on (128 units of 2000 rows at d = 128: 13.9 against 16.3; 48 units of
+    // 4000 rows: 12.5 against 11.1).
+    const int cta_tiles = p.units >= 96 ? 4 : (p.units >= 32 ? 2 : 1);
+    p.cta_units = p.units <= kSms && tiles <= cta_tiles * split_warps(p.nt);
+    p.warps = p.cta_units ? std::min(tiles, split_warps(p.nt)) : split_warps(p.nt);
+    p.ctas = p.cta_units ? static_cast<int>(p.units) : std::min(p.chunks, kSms);
+    p.combine = !p.cta_units && tiles > 1;
     return p;
 }
 size_t round_up(size_t n, size_t m) { return (n + m - 1) / m * m; }
@@ -914,17 +959,19 @@ cudaLaunchConfig_t pdl_config(dim3 grid, int threads, size_t smem, cudaStream_t 
 
 template <int D, int NT, int FO>
 cudaError_t launch_split_form(const Kv4Args& a, const SplitPlan& p, cudaStream_t s) {
-    constexpr size_t smem = split_warps(NT) * Kv4Geo<D>::WARP;
+    constexpr size_t most = split_warps(NT) * Kv4Geo<D>::WARP;
     const auto fn = kv4_split_kernel<D, NT, FO>;
     cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(smem));
+                                         static_cast<int>(most));
     if (e != cudaSuccess) return e;
     cudaLaunchAttribute attr;
-    const cudaLaunchConfig_t cfg = pdl_config(dim3(p.ctas, 1, 1), 32 * split_warps(NT), smem, s, &attr);
+    const cudaLaunchConfig_t cfg = pdl_config(dim3(p.ctas, 1, 1), 32 * p.warps, p.warps * Kv4Geo<D>::WARP, s, &attr);
     e = cudaLaunchKernelEx(&cfg, fn, a);
     if (e != cudaSuccess || !p.combine) return e;
     const unsigned rows = static_cast<unsigned>(a.n_seqs) * a.n_kv_heads * a.q_rows;
-    const cudaLaunchConfig_t ccfg = pdl_config(dim3(rows, 1, 1), 32 * kCombineWarps, 0, s, &attr);
+    // few rows have many records each (up to one a chunk): more warps for them
+    const int warps = rows <= 2 * kSms ? kCombineWarps : 4;
+    const cudaLaunchConfig_t ccfg = pdl_config(dim3(rows, 1, 1), 32 * warps, 0, s, &attr);
     return cudaLaunchKernelEx(&ccfg, kv4_combine_kernel<D, query_rows<NT, FO>()>, a);
 }
 
@@ -1042,6 +1089,7 @@ cudaError_t launch_kv4_attention(const alpaca_kv4_attn_desc& d, alpaca_attn_kern
         a.q_rows = p.q_rows;
         a.q_groups = p.q_groups;
         a.chunks = p.chunks;
+        a.cta_units = p.cta_units;
         if (p.combine) {
             a.plan = static_cast<int2*>(ws);
             a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + plan_bytes(p));
@@ -1049,7 +1097,7 @@ cudaError_t launch_kv4_attention(const alpaca_kv4_attn_desc& d, alpaca_attn_kern
         return d.head_dim == 128 ? launch_split<128>(a, p, s) : launch_split<64>(a, p, s);
     }
     a.q_rows = a.q_groups = 0;
-    a.chunks = 0;
+    a.chunks = a.cta_units = 0;
     const int64_t rows = static_cast<int64_t>(d.n_seqs) * d.tokens * d.n_heads;
     cudaLaunchAttribute attr;
     const cudaLaunchConfig_t cfg =
