@@ -510,12 +510,18 @@ alpaca_cuda_status validate_kv4_attn(const alpaca_kv4_attn_desc* dp) {
     return validate_kv4_cache(d.cache, d.n_seqs, d.n_kv_heads, d.head_dim, rows, "kv4_attention");
 }
 
+// The split kernel's time grows with the tokens, the prefill form's hardly below 128 of them (it decodes the whole context
+// first, and its tiles are 128 queries high). Both measured, us: 9/3 heads at d = 64, 4 x 4000 rows: 16 tokens 16.2 / 24.8, 64
+// tokens 30.6 / 26.2; 32/32 heads, 4 x 4000: 16 tokens 30 / 76, 64 tokens 88 / 76; 32/8 heads at d = 128, 4 x 4000: 16 tokens
+// 50 / 81, 32 tokens 91 / 81. Below the limit the results have f32 accuracy besides.
+constexpr int kKv4PrefillMinTokens = 32;
+
 bool kv4_fast_head_dim(const alpaca_kv4_attn_desc& d) { return d.head_dim == 64 || d.head_dim == 128; }
 
 alpaca_attn_kernel kv4_select(const alpaca_kv4_attn_desc& d) {
     if (d.flags & ALPACA_ATTN_FLAG_VARLEN) return ALPACA_ATTN_PREFILL_TC;
     if (!kv4_fast_head_dim(d)) return ALPACA_ATTN_GENERAL;
-    return (d.tokens >= kPrefillMinTokens && !d.ctx_lens) ? ALPACA_ATTN_PREFILL_TC : ALPACA_ATTN_DECODE_SPLIT;
+    return (d.tokens >= kKv4PrefillMinTokens && !d.ctx_lens) ? ALPACA_ATTN_PREFILL_TC : ALPACA_ATTN_DECODE_SPLIT;
 }
 
 // Descriptor checks, then the kernel choice (ALPACA_ATTN_AUTO resolved) and its limits.

@@ -44,7 +44,6 @@ struct Kv4Args {
     int2* plan;      // [unit]: the first chunk that holds tiles of it, and how many do
     float* partial;  // [chunk + unit][query row of the group][d + 4]: accumulators, m (log2 units), l
     int chunks;
-    int cta_units;   // one CTA per unit: its warps share the unit's tiles and meet in shared memory (no records)
     float scale;
     unsigned* err;
 };
@@ -182,7 +181,15 @@ __device__ __forceinline__ int next_page(const Kv4Args& a, Pages& p, int seq, in
         p.entry = p.b + lane < a.c.max_blocks ? a.c.block_table[static_cast<int64_t>(seq) * a.c.max_blocks + p.b + lane] : -1;
     }
     const int blk = __shfl_sync(0xffffffffu, p.entry, p.b - p.base);
-    for (p.r += step * Kv4Geo<D>::TK; p.r >= a.c.rows; p.r -= a.c.rows) p.b++;
+    p.r += step * Kv4Geo<D>::TK;
+    if (step == 1) {
+        if (p.r >= a.c.rows) {
+            p.r = 0;
+            p.b++;
+        }
+    } else {
+        for (; p.r >= a.c.rows; p.r -= a.c.rows) p.b++;
+    }
     if (blk >= 0 && blk < a.c.pool_blocks) return blk;
     atomicOr(a.err, kDevErrBadIndex);
     return -1;
@@ -604,7 +611,8 @@ __device__ __forceinline__ void load_queries(const Kv4Args& a, int seq, int kvh,
 // Warps of a CTA, one CTA per SM: as many as the registers of the form allow (128, 168 and 255 a thread).
 __host__ __device__ constexpr int split_warps(int NT) { return NT == 4 ? 8 : (NT == 2 ? 12 : 16); }
 
-template <int D, int NT, int FO>
+// kCta: one CTA per unit; its warps share the unit's tiles and meet in shared memory (no records).
+template <int D, int NT, int FO, bool kCta>
 __global__ void __launch_bounds__(32 * split_warps(NT), 1) kv4_split_kernel(const __grid_constant__ Kv4Args a) {
     using Ge = Kv4Geo<D>;
     constexpr int QR = query_rows<NT, FO>();
@@ -618,7 +626,7 @@ __global__ void __launch_bounds__(32 * split_warps(NT), 1) kv4_split_kernel(cons
     const uint32_t ring_u32 = smem_u32(ring);
     const int chunk = warp * gridDim.x + blockIdx.x;  // a call with few chunks spreads them over the SMs
     Chunk w;
-    if (a.cta_units) {
+    if constexpr (kCta) {
         const int hg = a.n_kv_heads * a.q_groups;
         w.seq = blockIdx.x / hg;
         w.head_group = blockIdx.x - w.seq * hg;
@@ -629,15 +637,15 @@ __global__ void __launch_bounds__(32 * split_warps(NT), 1) kv4_split_kernel(cons
         if (w.begin >= w.end) return;
     }
     const int64_t chunk_begin = w.begin;
-    const int step = a.cta_units ? blockDim.x / 32 : 1;
+    const int step = kCta ? blockDim.x / 32 : 1;
     while (true) {  // the units of the chunk
         const int seq = w.seq, kvh = w.head_group / a.q_groups, qg = w.head_group - kvh * a.q_groups, L = w.L;
         const int r0 = qg * QR, r_last = min(r0 + QR, a.q_rows) - 1;
         const int64_t tile0 = w.first + kUnitCost;  // place of the unit's first tile
         const int ut = unit_tiles<D>(L);
-        const int t0 = a.cta_units ? warp : static_cast<int>(max(w.begin - tile0, static_cast<int64_t>(0)));
-        const int t1 = a.cta_units ? ut : static_cast<int>(min(static_cast<int64_t>(ut), w.end - tile0));
-        if (!a.cta_units && t1 <= t0) return;  // the chunk ends in the places before the unit's first tile
+        const int t0 = kCta ? warp : static_cast<int>(max(w.begin - tile0, static_cast<int64_t>(0)));
+        const int t1 = kCta ? ut : static_cast<int>(min(static_cast<int64_t>(ut), w.end - tile0));
+        if (!kCta && t1 <= t0) return;  // the chunk ends in the places before the unit's first tile
         // rows that query row q sees: L - tokens + 1 + its token; the last one's bounds the rows worth reading
         const int min_lim = L - a.tokens + 1 + r0 / a.group;
         const int row_end = min(L, L - a.tokens + 1 + r_last / a.group);
@@ -669,14 +677,14 @@ __global__ void __launch_bounds__(32 * split_warps(NT), 1) kv4_split_kernel(cons
         // A unit that lies wholly in this chunk is finished here, else its part goes to a record. Parts are numbered chunk +
         // unit: along the row of places every next part has a higher number, and a unit's parts follow one another. With one CTA
         // per unit the parts are its warps', in shared memory over the rings.
-        const bool whole = !a.cta_units && t1 - t0 == ut;
+        const bool whole = !kCta && t1 - t0 == ut;
         const int64_t unit = static_cast<int64_t>(seq) * a.n_kv_heads * a.q_groups + w.head_group;
-        if (!a.cta_units && t0 == 0 && lane == 0 && a.plan) {
+        if (!kCta && t0 == 0 && lane == 0 && a.plan) {
             a.plan[unit] = make_int2(chunk, static_cast<int>(div_pos(tile0 - chunk_begin + ut - 1, w.size)) + 1);
         }
-        float* rec0 = a.cta_units ? reinterpret_cast<float*>(smem) + warp * QR * Ge::REC : a.partial + (chunk + unit) * QR * Ge::REC;
+        float* rec0 = kCta ? reinterpret_cast<float*>(smem) + warp * QR * Ge::REC : a.partial + (chunk + unit) * QR * Ge::REC;
         static_assert(sizeof(float) * QR * Ge::REC <= Ge::WARP, "a warp's record must fit its ring");
-        if (a.cta_units) __syncthreads();  // every warp is done with its ring
+        if (kCta) __syncthreads();  // every warp is done with its ring
         else __syncwarp();                 // the next unit's copies go to stages that every lane has read
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
@@ -710,7 +718,7 @@ __global__ void __launch_bounds__(32 * split_warps(NT), 1) kv4_split_kernel(cons
             if (!whole && g == 0)
                 *reinterpret_cast<float2*>(rec0 + row * Ge::REC + D) = make_float2(s.m[nt] == -INFINITY ? -INFINITY : s.fs[nt] * s.m[nt], l);
         }
-        if (a.cta_units) {
+        if constexpr (kCta) {
             __syncthreads();
             const int warps = min(step, max(row_end > 0 ? (row_end + Ge::TK - 1) / Ge::TK : 0, 1));  // those with tiles
             for (int i = threadIdx.x; i < QR * D; i += blockDim.x) {
@@ -742,16 +750,15 @@ __global__ void __launch_bounds__(32 * split_warps(NT), 1) kv4_split_kernel(cons
 
 // ------------------------------------------------------------------------------------------------ combine
 
-constexpr int kCombineWarps = 16;  // at most
-constexpr int kCombineHeld = 4;    // records a warp has in flight
+constexpr int kCombineHeld = 4;  // records a warp has in flight
 
-// One CTA per query row: its warps share the records of the row's unit, each with a running maximum.
-template <int D, int QR>
-__global__ void __launch_bounds__(32 * kCombineWarps) kv4_combine_kernel(const __grid_constant__ Kv4Args a) {
+// One CTA per query row: its W warps share the records of the row's unit, each with a running maximum.
+template <int D, int QR, int W>
+__global__ void __launch_bounds__(32 * W) kv4_combine_kernel(const __grid_constant__ Kv4Args a) {
     constexpr int EPL = D / 32, REC = Kv4Geo<D>::REC;
-    __shared__ float s_acc[kCombineWarps][D];
-    __shared__ float s_ml[kCombineWarps][2];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x / 32;
+    __shared__ float s_acc[W][D];
+    __shared__ float s_ml[W][2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rr = blockIdx.x % a.q_rows, kvh = (blockIdx.x / a.q_rows) % a.n_kv_heads, seq = blockIdx.x / (a.q_rows * a.n_kv_heads);
     const int64_t unit = (static_cast<int64_t>(seq) * a.n_kv_heads + kvh) * a.q_groups + rr / QR;
     // Every CTA waits for the split grid, so that a later launch which sees this grid complete sees the split kernel's
@@ -768,12 +775,12 @@ __global__ void __launch_bounds__(32 * kCombineWarps) kv4_combine_kernel(const _
     float m = -INFINITY, l = 0.f, acc[EPL];
 #pragma unroll
     for (int e = 0; e < EPL; e++) acc[e] = 0.f;
-    for (int i0 = warp; i0 < part.y; i0 += warps * kCombineHeld) {
+    for (int i0 = warp; i0 < part.y; i0 += W * kCombineHeld) {
         float2 ml[kCombineHeld];
         float v[kCombineHeld][EPL];
 #pragma unroll
         for (int k = 0; k < kCombineHeld; k++) {
-            const int i = i0 + k * warps;
+            const int i = i0 + k * W;
             const float* p = base + static_cast<int64_t>(i) * QR * REC;
             ml[k] = make_float2(-INFINITY, 0.f);
 #pragma unroll
@@ -810,10 +817,12 @@ __global__ void __launch_bounds__(32 * kCombineWarps) kv4_combine_kernel(const _
     }
     __syncthreads();
     float M = -INFINITY;
-    for (int w = 0; w < warps; w++) M = fmaxf(M, s_ml[w][0]);
-    for (int col = threadIdx.x; col < D; col += blockDim.x) {
+#pragma unroll
+    for (int w = 0; w < W; w++) M = fmaxf(M, s_ml[w][0]);
+    for (int col = threadIdx.x; col < D; col += 32 * W) {
         float o = 0.f, sum = 0.f;
-        for (int w = 0; w < warps; w++) {
+#pragma unroll
+        for (int w = 0; w < W; w++) {
             const float f = s_ml[w][0] == -INFINITY ? 1.f : ex2_approx(s_ml[w][0] - M);
             o = fmaf(s_acc[w][col], f, o);
             sum = fmaf(s_ml[w][1], f, sum);
@@ -957,10 +966,10 @@ cudaLaunchConfig_t pdl_config(dim3 grid, int threads, size_t smem, cudaStream_t 
     return cfg;
 }
 
-template <int D, int NT, int FO>
+template <int D, int NT, int FO, bool kCta>
 cudaError_t launch_split_form(const Kv4Args& a, const SplitPlan& p, cudaStream_t s) {
     constexpr size_t most = split_warps(NT) * Kv4Geo<D>::WARP;
-    const auto fn = kv4_split_kernel<D, NT, FO>;
+    const auto fn = kv4_split_kernel<D, NT, FO, kCta>;
     cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          static_cast<int>(most));
     if (e != cudaSuccess) return e;
@@ -970,9 +979,14 @@ cudaError_t launch_split_form(const Kv4Args& a, const SplitPlan& p, cudaStream_t
     if (e != cudaSuccess || !p.combine) return e;
     const unsigned rows = static_cast<unsigned>(a.n_seqs) * a.n_kv_heads * a.q_rows;
     // few rows have many records each (up to one a chunk): more warps for them
-    const int warps = rows <= 2 * kSms ? kCombineWarps : 4;
+    constexpr int QR = query_rows<NT, FO>();
+    const int warps = rows <= 2 * kSms ? 16 : 4;
     const cudaLaunchConfig_t ccfg = pdl_config(dim3(rows, 1, 1), 32 * warps, 0, s, &attr);
-    return cudaLaunchKernelEx(&ccfg, kv4_combine_kernel<D, query_rows<NT, FO>()>, a);
+    return warps == 16 ? cudaLaunchKernelEx(&ccfg, kv4_combine_kernel<D, QR, 16>, a) : cudaLaunchKernelEx(&ccfg, kv4_combine_kernel<D, QR, 4>, a);
+}
+template <int D, int NT, int FO>
+cudaError_t launch_split_form(const Kv4Args& a, const SplitPlan& p, cudaStream_t s) {
+    return p.cta_units ? launch_split_form<D, NT, FO, true>(a, p, s) : launch_split_form<D, NT, FO, false>(a, p, s);
 }
 
 template <int D>
@@ -1089,7 +1103,6 @@ cudaError_t launch_kv4_attention(const alpaca_kv4_attn_desc& d, alpaca_attn_kern
         a.q_rows = p.q_rows;
         a.q_groups = p.q_groups;
         a.chunks = p.chunks;
-        a.cta_units = p.cta_units;
         if (p.combine) {
             a.plan = static_cast<int2*>(ws);
             a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + plan_bytes(p));
@@ -1097,7 +1110,7 @@ cudaError_t launch_kv4_attention(const alpaca_kv4_attn_desc& d, alpaca_attn_kern
         return d.head_dim == 128 ? launch_split<128>(a, p, s) : launch_split<64>(a, p, s);
     }
     a.q_rows = a.q_groups = 0;
-    a.chunks = a.cta_units = 0;
+    a.chunks = 0;
     const int64_t rows = static_cast<int64_t>(d.n_seqs) * d.tokens * d.n_heads;
     cudaLaunchAttribute attr;
     const cudaLaunchConfig_t cfg =

@@ -282,6 +282,15 @@ ATTN = [
     (2, 5, 8, 1, 128, [4, 200], 0),
     (2, 33, 4, 2, 64, [20, 150], 0),
     (1, 9, 6, 2, 128, [9], 0),
+    # one and two query rows per KV head (folded columns), contexts past one tile a warp, paged
+    (3, 1, 4, 4, 128, [1, 40, 700], 48),
+    (3, 1, 4, 4, 64, [16, 65, 1300], 16),
+    (3, 2, 3, 3, 64, [1, 130, 999], 0),
+    (2, 1, 4, 2, 128, [100, 601], 128),
+    # one CTA per unit with several tiles a warp (32 and 96 units or more), and its limits
+    (17, 1, 6, 2, 64, [7 * i * i for i in range(17)], 0),
+    (49, 1, 4, 2, 64, [60 + 70 * i for i in range(49)], 64),
+    (33, 3, 8, 4, 128, [40 * i for i in range(33)], 0),
 ]
 
 
@@ -424,8 +433,7 @@ def test_prefill(cuda_lib, d, H, Hkv, T, ctx, block_rows, types):
         table = dev(tb)
     out = torch.full((S, T, H, d), float("nan"), dtype=DT[out_type], device="cuda")
     cache = to_gpu(parts)
-    desc = ab.kv4_attention(dev(q).to(DT[q_type]), cache, out, start_position=ctx - T, block_table=table)
-    assert ab.kv4_select(desc) == ab.Kernel.PREFILL_TC
+    ab.kv4_attention(dev(q).to(DT[q_type]), cache, out, start_position=ctx - T, block_table=table, kind=ab.Kernel.PREFILL_TC)
     ab.device_status()
     rows = sorted({0, 1, T // 2, T - 1})
     for s in range(S):
@@ -461,3 +469,32 @@ def test_prefill_ragged(cuda_lib, block_rows):
         if counts[s]:
             want = _kv4.attention(q[offs[s]:offs[s + 1]], k[s], v[s], starts[s] + counts[s])
             check(got[offs[s]:offs[s + 1]], want, TC_TOL, "f32")
+
+
+def test_rotation_at_long_positions(cuda_lib):
+    """Angles far out: cos and sin keep double accuracy before their one rounding, as the oracle's."""
+    import alpaca_b200 as ab
+    rng = np.random.default_rng(29)
+    for start in (100_000, 12_345_678, (1 << 30) - 8):
+        for d in (64, 96):
+            q = rng.standard_normal((1, 4, 2, d)).astype(np.float32)
+            out = torch.empty((1, 4, 2, d), dtype=torch.float32, device="cuda")
+            ab.qkv_append(dev(q), None, None, out, None, theta=500000.0, start_position=start, interleaved=bool(d == 64))
+            ab.device_status()
+            assert np.array_equal(out[0].cpu().numpy(), oracle.rope(q[0], start, 500000.0, bool(d == 64)))
+
+
+def test_example_session(cuda_lib, capsys):
+    """The session of examples/kv4_session.py: the caches' bytes, and 4-bit context vectors near the f16 cache's.
+    A value is off by at most half a step, uniform over it: 1 / sqrt(12) of a step of about 4.1 / 15 standard deviations, 8%; the
+    scores' and the values' errors together stay below twice that."""
+    import importlib.util
+    from pathlib import Path
+    path = Path(__file__).resolve().parent.parent / "examples" / "kv4_session.py"
+    spec = importlib.util.spec_from_file_location("kv4_session", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    r = mod.main(["--prompt", "300", "--tokens", "5", "--chunk", "128", "--layers", "2"])
+    rows = 305  # 2 layers, K and V, 3 heads of 64: 128 bytes a head row, and 36 with the rows rounded up to 16
+    assert r["bytes"] == {"f16": 2 * 2 * 3 * 128 * rows, "4-bit": 2 * 2 * 3 * 36 * 320}
+    assert r["relative_error"] < 0.16

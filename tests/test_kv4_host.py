@@ -217,7 +217,8 @@ def test_kernel_choice(lib):
     wide = dict(q_seq_stride=64 * 9 * 64, out_seq_stride=64 * 9 * 64)
     assert ab.kv4_select(attn_desc()) == K.DECODE_SPLIT
     assert ab.kv4_select(attn_desc(tokens=7, start_position=100, **wide)) == K.DECODE_SPLIT
-    assert ab.kv4_select(attn_desc(tokens=64, start_position=100, **wide)) == K.PREFILL_TC
+    assert ab.kv4_select(attn_desc(tokens=31, start_position=100, **wide)) == K.DECODE_SPLIT
+    assert ab.kv4_select(attn_desc(tokens=32, start_position=100, **wide)) == K.PREFILL_TC
     assert ab.kv4_select(attn_desc(tokens=64, ctx_lens=FAKE, max_ctx_len=200, **wide)) == K.DECODE_SPLIT
     assert ab.kv4_select(attn_desc(head_dim=96, q_token_stride=864, out_token_stride=864, q_seq_stride=864, out_seq_stride=864)) == K.GENERAL
     varlen = attn_desc(flags=1, q_offsets=FAKE, start_positions=FAKE, total_tokens=5, max_ctx_len=9)
