@@ -636,7 +636,9 @@ def kv4_prefill_varlen(q: torch.Tensor, cache: Kv4Cache, out: torch.Tensor, q_of
 def _kv4_run(desc: Kv4AttnDesc, kind: Kernel, workspace: torch.Tensor | None, device, stream) -> None:
     need = kv4_workspace_bytes(desc, kind)
     if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
-        # allocated on the stream that uses it, so that its memory is not handed out again before the call has run
-        with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(device)):
+        if stream is None:
             workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        else:  # allocated on the stream that uses it, so that its memory is not handed out again before the call has run
+            with torch.cuda.stream(stream):
+                workspace = torch.empty(need, dtype=torch.uint8, device=device)
     kv4_attention_launch(desc, workspace, kind, stream)

@@ -2,8 +2,8 @@
 
 Per layer and step a model does: new tokens' projections -> head norms + RoPE + cache append (one pass) -> attention over the
 cache. Here the projections are seeded random numbers of a SmolLM2-135M layer's shape; the prompt goes through in chunks, then
-tokens one by one. Prints the caches' bytes, the time of a decode step, and how far the 4-bit session's context vectors are from
-the f16 session's.
+tokens one by one. Prints the caches' bytes, the time of a decode step as this loop issues it (at these sizes mostly the host's:
+descriptors and launches), and how far the 4-bit session's context vectors are from the f16 session's.
 
     python examples/kv4_session.py [--prompt 1000] [--tokens 32] [--chunk 512] [--layers 4]
 """
@@ -33,6 +33,7 @@ class Session:
             self.caches = [tuple(torch.zeros((1, rows, KV_HEADS, HEAD_DIM), dtype=torch.float16, device="cuda") for _ in range(2))
                            for _ in range(layers)]
         self.position = 0
+        self.workspace = None  # of the attention calls: the largest asked for so far, shared by the layers
 
     def bytes(self) -> int:
         return sum(t.numel() * t.element_size() for c in self.caches for t in c)
@@ -45,7 +46,11 @@ class Session:
             ab.qkv_append(q, k, v, q_rot, cache, theta=THETA, start_position=self.position, q_norm=self.norms[0], k_norm=self.norms[1])
             out = torch.empty_like(q_rot)
             if self.four_bit:
-                ab.kv4_attention(q_rot, cache, out, start_position=self.position)
+                desc = ab.make_kv4_attn_desc(q_rot, cache, out, start_position=self.position)
+                need = ab.kv4_workspace_bytes(desc)
+                if self.workspace is None or self.workspace.nbytes < need:
+                    self.workspace = torch.empty(need, dtype=torch.uint8, device="cuda")
+                ab.kv4_attention_launch(desc, self.workspace)
             else:
                 ab.attention_device(q_rot, cache[0], cache[1], out, start_position=self.position)
             outs.append(out)
