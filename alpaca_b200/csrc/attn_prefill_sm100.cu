@@ -183,10 +183,10 @@ __device__ __forceinline__ Item decode_item(const PrefillArgs& a, int it) {
         const int unit = KS ? slot / a.kv_splits : slot;
         const int part = KS ? slot - unit * a.kv_splits : 0;
         x.head = it - slot * a.n_heads;
-        const int4 r = __ldg(a.plan + 1 + 2 * unit);
+        const int4 r = a.plan[1 + 2 * unit];
         x.seq = r.x;
         x.cseq = 0;
-        x.ctx_end = __ldg(a.plan + 2 + 2 * unit).x;
+        x.ctx_end = a.plan[2 + 2 * unit].x;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             x.row0[t] = r.y + t * kBM;
@@ -247,7 +247,7 @@ __device__ __forceinline__ TileWork tile_work(const PrefillArgs& a, int it, int 
         const int unit = KS ? slot / a.kv_splits : slot;
         const int part = KS ? slot - unit * a.kv_splits : 0;
         w.head = it - slot * a.n_heads;
-        const int4 r = __ldg(a.plan + 1 + 2 * unit);
+        const int4 r = a.plan[1 + 2 * unit];
         w.seq = r.x;
         w.cseq = 0;
         w.row0 = r.y + t * kBM;
@@ -407,8 +407,10 @@ __global__ void __launch_bounds__(threads_for<R, NT>(), 1)
     // kernel on the stream drains; no global memory is touched before its writes are complete and visible.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t tmem_base = sm->tmem_base;
-    // Work items: fixed by the call's shape, or (ragged form) units of the plan the previous launch wrote x heads.
-    const int total_items = VL ? __ldg(&a.plan[0].x) * a.n_heads * (KS ? a.kv_splits : 1) : a.total_items;
+    // Work items: fixed by the call's shape, or (ragged form) units of the plan the previous launch wrote x heads. What
+    // earlier launches of the call wrote is read with plain loads: __ldg may be moved above griddepcontrol.wait, since
+    // it promises that nothing writes the memory while the kernel lives.
+    const int total_items = VL ? a.plan[0].x * a.n_heads * (KS ? a.kv_splits : 1) : a.total_items;
     if (warp == 0) {
         if constexpr (R == 2 || NT == 3) setmaxnreg_dec<kRegsControl>();
         if (lane != 0) return;
@@ -1083,7 +1085,8 @@ __global__ void __launch_bounds__(threads_for<R, NT>(), 1)
 template <int D, int BN, bool VL>
 __global__ void __launch_bounds__(256) prefill_merge_kernel(const PrefillArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // every part of the prefill launch has been written
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // every part of the prefill launch has been written (plain loads
+                                                        // below: __ldg may be moved above the wait)
     constexpr int NT = 2, CPL = D / 32;                  // columns per lane
     const int w = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int row = w % kBM, tile = (w / kBM) % NT, base = w / (kBM * NT);
@@ -1094,8 +1097,8 @@ __global__ void __launch_bounds__(256) prefill_merge_kernel(const PrefillArgs a)
     if constexpr (VL) {
         // base = (unit, head) of the ragged work list (unit-major, head-minor, as the prefill kernel deals it)
         const int unit = base / a.n_heads, head = base - unit * a.n_heads;
-        if (unit >= __ldg(&a.plan[0].x)) return;
-        const int4 r = __ldg(a.plan + 1 + 2 * unit);
+        if (unit >= a.plan[0].x) return;
+        const int4 r = a.plan[1 + 2 * unit];
         const int rows_t = max(0, min(kBM, r.w - tile * kBM));
         if (row >= rows_t) return;
         nblk = (r.z + tile * kBM + rows_t + BN - 1) / BN;
@@ -1140,11 +1143,11 @@ __global__ void __launch_bounds__(256) prefill_merge_kernel(const PrefillArgs a)
         for (int c = 0; c < CPL; c++) op[p][c] = 0.f;
         if (use) {
             const float* rec = a.part + ((item0 + p * pstep) * NT + tile) * kBM * (D + 2) + row * (D + 2);
-            const float2 ml = __ldg(reinterpret_cast<const float2*>(rec + D));
+            const float2 ml = *reinterpret_cast<const float2*>(rec + D);
             mp[p] = ml.x;
             lp[p] = ml.y;
 #pragma unroll
-            for (int c = 0; c < CPL; c++) op[p][c] = __ldg(rec + lane + 32 * c);
+            for (int c = 0; c < CPL; c++) op[p][c] = rec[lane + 32 * c];
         }
     }
     float M = -INFINITY;
