@@ -463,7 +463,8 @@ __global__ void __launch_bounds__(kReadThreads) kv4_read_kernel(const __grid_con
 #pragma unroll
     for (int b = 0; b < kReadBatch; b++) {
         const int64_t i = static_cast<int64_t>(blockIdx.x) * kReadRows + b * (kReadThreads / 4) + threadIdx.x / 4;
-        const int row = static_cast<int>(i / a.n_kv_heads), head = static_cast<int>(i - static_cast<int64_t>(row) * a.n_kv_heads);
+        const int row = static_cast<int>(i >> 32 ? i / a.n_kv_heads : static_cast<uint32_t>(i) / static_cast<uint32_t>(a.n_kv_heads));
+        const int head = static_cast<int>(i - static_cast<int64_t>(row) * a.n_kv_heads);
         at[b] = -1;
 #pragma unroll
         for (int k = 0; k < NB; k++) w[b][k] = h[b][k] = 0;

@@ -372,7 +372,7 @@ def _stream_handle(stream: torch.cuda.Stream | None) -> int:
     """cudaStream_t of `stream`, or of torch's current stream (without building a Stream object: 3 us a call)."""
     if stream is not None:
         return stream.cuda_stream
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 class Kv4Cache(NamedTuple):
@@ -494,7 +494,9 @@ def make_qkv_desc(q: torch.Tensor | None, k: torch.Tensor | None, v: torch.Tenso
 
 
 def qkv_launch(desc: QkvDesc, stream: torch.cuda.Stream | None = None) -> None:
-    check(load().alpaca_qkv_append(ctypes.byref(desc), _stream_handle(stream)))
+    status = load().alpaca_qkv_append(ctypes.byref(desc), _stream_handle(stream))
+    if status:
+        check(status)
 
 
 def qkv_append(q: torch.Tensor | None, k: torch.Tensor | None, v: torch.Tensor | None, q_out: torch.Tensor | None,
@@ -531,7 +533,9 @@ def make_kv4_read_desc(cache: Kv4Cache, k_out: torch.Tensor, v_out: torch.Tensor
 
 
 def kv4_read_launch(desc: Kv4ReadDesc, stream: torch.cuda.Stream | None = None) -> None:
-    check(load().alpaca_kv4_read(ctypes.byref(desc), _stream_handle(stream)))
+    status = load().alpaca_kv4_read(ctypes.byref(desc), _stream_handle(stream))
+    if status:
+        check(status)
 
 
 def kv4_read(cache: Kv4Cache, k_out: torch.Tensor, v_out: torch.Tensor, *, start_row: int = 0,
@@ -607,7 +611,9 @@ def kv4_attention_launch(desc: Kv4AttnDesc, workspace: torch.Tensor | None = Non
     """Enqueue one call of alpaca_kv4_attention on `stream` (default: torch's current stream)."""
     ws_ptr = workspace.data_ptr() if workspace is not None else None
     ws_len = workspace.nbytes if workspace is not None else 0
-    check(load().alpaca_kv4_attention(ctypes.byref(desc), kind, ws_ptr, ws_len, _stream_handle(stream)))
+    status = load().alpaca_kv4_attention(ctypes.byref(desc), kind, ws_ptr, ws_len, _stream_handle(stream))
+    if status:
+        check(status)
 
 
 def kv4_attention(q: torch.Tensor, cache: Kv4Cache, out: torch.Tensor, *, start_position: int = 0,

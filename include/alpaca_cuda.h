@@ -427,8 +427,8 @@ alpaca_cuda_status alpaca_kv4_read(const alpaca_kv4_read_desc* desc, alpaca_stre
  * Kernels (alpaca_attn_kernel): DECODE_SPLIT (head_dim 64 / 128, any token count: a few tokens over long contexts; f32
  * accuracy), PREFILL_TC (head_dim 64 / 128, uniform start_position or VARLEN: the visible rows are decoded to f16 in the
  * workspace, exactly, and the tensor-core prefill runs over them with its accuracy, P rounded to f16), GENERAL (any
- * head_dim). AUTO: PREFILL_TC for VARLEN and for 32 or more tokens at a uniform position, else DECODE_SPLIT, else GENERAL
- * for other head dims. */
+ * head_dim). AUTO: PREFILL_TC for VARLEN; DECODE_SPLIT with ctx_lens; for a uniform position the one of the two that is
+ * estimated faster (DECODE_SPLIT below some 32 to 128 tokens); GENERAL for other head dims. */
 typedef struct alpaca_kv4_attn_desc {
     int32_t n_seqs;          /* 1 .. 65535 */
     int32_t n_heads;

@@ -498,3 +498,35 @@ def test_example_session(cuda_lib, capsys):
     rows = 305  # 2 layers, K and V, 3 heads of 64: 128 bytes a head row, and 36 with the rows rounded up to 16
     assert r["bytes"] == {"f16": 2 * 2 * 3 * 128 * rows, "4-bit": 2 * 2 * 3 * 36 * 320}
     assert r["relative_error"] < 0.16
+
+
+@pytest.mark.parametrize("d", [64, 96, 128])
+def test_offsets_past_32_bits(cuda_lib, d):
+    """Two sequences whose caches lie more than 2^32 bytes (and 2^31 scales) apart: append, read-back and every attention form."""
+    import alpaca_b200 as ab
+    rng = np.random.default_rng(31)
+    S, T, H, Hkv, rows = 2, 40, 4, 2, 48
+    far = (1 << 32) + 4096
+    codes, scales = torch.zeros(far + 2 * Hkv * rows * d, dtype=torch.uint8, device="cuda"), \
+        torch.zeros(far + 2 * Hkv * rows * (d // 32) + 4096, dtype=torch.int16, device="cuda")
+
+    def view(buf, width, first):
+        return buf.as_strided((S, Hkv, rows, width), (far, rows * width, width, 1), first)
+    cache = ab.Kv4Cache(view(codes, d // 2, 0), view(scales, d // 32, 0), view(codes, d // 2, Hkv * rows * d // 2),
+                        view(scales, d // 32, Hkv * rows * (d // 32)))
+    q, k, v = (rng.standard_normal((S, T, h, d)).astype(np.float32) for h in (H, Hkv, Hkv))
+    rot = torch.empty((S, T, H, d), dtype=torch.float32, device="cuda")
+    ab.qkv_append(dev(q), dev(k), dev(v), rot, cache, theta=1e4)
+    ko, vo = (torch.empty((S, T, Hkv, d), dtype=torch.float32, device="cuda") for _ in range(2))
+    ab.kv4_read(cache, ko, vo)
+    ab.device_status()
+    want_v = _kv4.values(*_kv4.quantise(v))
+    assert np.array_equal(vo.double().cpu().numpy(), want_v)
+    kd, qd = ko.double().cpu().numpy(), rot.cpu().numpy()
+    for kind in (["DECODE_SPLIT", "PREFILL_TC", "GENERAL"] if d != 96 else ["GENERAL"]):
+        out = torch.empty((S, T, H, d), dtype=torch.float32, device="cuda")
+        ab.kv4_attention(rot, cache, out, kind=ab.Kernel[kind])
+        ab.device_status()
+        for s in range(S):
+            want = _kv4.attention(qd[s], np.swapaxes(kd[s], 0, 1), np.swapaxes(want_v[s], 0, 1), T)
+            check(out[s].cpu().numpy(), want, TC_TOL if kind == "PREFILL_TC" else F32_TOL, "f32")

@@ -214,12 +214,15 @@ def test_an_empty_read_is_ok(lib):
 def test_kernel_choice(lib):
     import alpaca_b200 as ab
     K = ab.Kernel
-    wide = dict(q_seq_stride=64 * 9 * 64, out_seq_stride=64 * 9 * 64)
+    wide = dict(q_seq_stride=128 * 9 * 64, out_seq_stride=128 * 9 * 64)
     assert ab.kv4_select(attn_desc()) == K.DECODE_SPLIT
     assert ab.kv4_select(attn_desc(tokens=7, start_position=100, **wide)) == K.DECODE_SPLIT
-    assert ab.kv4_select(attn_desc(tokens=31, start_position=100, **wide)) == K.DECODE_SPLIT
-    assert ab.kv4_select(attn_desc(tokens=32, start_position=100, **wide)) == K.PREFILL_TC
-    assert ab.kv4_select(attn_desc(tokens=64, ctx_lens=FAKE, max_ctx_len=200, **wide)) == K.DECODE_SPLIT
+    assert ab.kv4_select(attn_desc(tokens=128, start_position=100, **wide)) == K.PREFILL_TC
+    # 4 sequences of 4000 rows: a few tokens on the split kernel, a chunk on the prefill
+    for tokens, kind in ((8, K.DECODE_SPLIT), (32, K.DECODE_SPLIT), (128, K.PREFILL_TC), (512, K.PREFILL_TC)):
+        big = dict(tokens=tokens, start_position=4000 - tokens, q_seq_stride=tokens * 576, out_seq_stride=tokens * 576)
+        assert ab.kv4_select(attn_desc(cache=cache_desc(rows=4000), **big)) == kind, tokens
+    assert ab.kv4_select(attn_desc(tokens=128, ctx_lens=FAKE, max_ctx_len=200, **wide)) == K.DECODE_SPLIT
     assert ab.kv4_select(attn_desc(head_dim=96, q_token_stride=864, out_token_stride=864, q_seq_stride=864, out_seq_stride=864)) == K.GENERAL
     varlen = attn_desc(flags=1, q_offsets=FAKE, start_positions=FAKE, total_tokens=5, max_ctx_len=9)
     assert ab.kv4_select(varlen) == K.PREFILL_TC
