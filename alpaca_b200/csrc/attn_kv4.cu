@@ -9,8 +9,8 @@
 //                  columns) and O^T = V^T P^T (16 channels x 8 columns). A column pair is one query row: f16 high part and
 //                  f16 remainder of q or p, so the f32 sum of the pair's two accumulators carries ~22 bits. Scores,
 //                  maxima and sums of a query row then live in the same lanes as its outputs (lane % 4).
-//                  K: codes enter as f16 denormals (c * 2^-24 and (c + 16 c') * 2^-24, one operation per pair; the queries'
-//                  combinations undo it), exact; a block's step and zero point are applied to the block's partial
+//                  K: codes enter as f16 denormals (c * 2^-24, one AND per pair; codes in bits 4-7 count 16 times, which
+//                  the queries' halves undo), exact; a block's step and zero point are applied to the block's partial
 //                  score in f32: s = sum_b step_b (acc_b - zero_b * qsum_b).
 //                  V: ldmatrix with transposition sets two keys' codes side by side; (c - zero) * step is exact in f16 (kv4.cuh).
 //                  P moves from accumulator to operand layout with movmatrix (no shared memory).
@@ -330,10 +330,9 @@ __device__ __forceinline__ void compute_tile(const uint8_t* st, const float4* s_
             }
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                // c_i and c_i + 16 c_(i+1) of both halves of a word: four operations for eight codes
-                const uint32_t a0[4] = {w[0][b] & 0x000F000Fu, w[1][b] & 0x000F000Fu, w[0][b] & 0x00FF00FFu, w[1][b] & 0x00FF00FFu};
-                const uint32_t x0 = __byte_perm(w[0][b], 0u, 0x4341), x1 = __byte_perm(w[1][b], 0u, 0x4341);
-                const uint32_t a1[4] = {x0 & 0x000F000Fu, x1 & 0x000F000Fu, x0, x1};
+                const uint32_t a0[4] = {w[0][b] & 0x000F000Fu, w[1][b] & 0x000F000Fu, w[0][b] & 0x00F000F0u, w[1][b] & 0x00F000F0u};
+                const uint32_t x0 = w[0][b] >> 8, x1 = w[1][b] >> 8;
+                const uint32_t a1[4] = {x0 & 0x000F000Fu, x1 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x00F000F0u};
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
                     if (f == 0) mma16816_first(acc[b][nt], a0, s.qb[f][nt][b][0], s.qb[f][nt][b][1]);
@@ -596,13 +595,9 @@ __device__ __forceinline__ void load_queries(const Kv4Args& a, int seq, int kvh,
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
             s.qsum[nt][b] = __shfl_sync(0xffffffffu, sum, src);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                // nibble pair (i, i + 4). Operands of even i are the codes c_i, those of odd i c_(i-1) + 16 c_i:
-                // q_0 c_0 + q_1 c_1 = (q_0 - q_1 / 16) c_0 + (q_1 / 16) (c_0 + 16 c_1)
-                const float y0 = (i & 1) ? x[b][i] * 0.0625f : fmaf(x[b][i + 1], -0.0625f, x[b][i]);
-                const float y1 = (i & 1) ? x[b][i + 4] * 0.0625f : fmaf(x[b][i + 5], -0.0625f, x[b][i + 4]);
+            for (int i = 0; i < 4; i++) {  // nibble pair (i, i + 4); codes of odd i count 16 times
                 uint32_t u, v;
-                split_f16_pair(y0, y1, u, v);
+                split_f16_pair(x[b][i] * ((i & 1) ? 0.0625f : 1.f), x[b][i + 4] * ((i & 1) ? 0.0625f : 1.f), u, v);
                 const uint32_t q = __byte_perm(u, v, (g & 1) ? 0x7632 : 0x5410);
 #pragma unroll
                 for (int f = 0; f < FO; f++) s.qb[f][nt][b][i] = FO == 1 || (g >> 1) / QP == f ? q : 0u;
