@@ -530,3 +530,83 @@ def test_offsets_past_32_bits(cuda_lib, d):
         for s in range(S):
             want = _kv4.attention(qd[s], np.swapaxes(kd[s], 0, 1), np.swapaxes(want_v[s], 0, 1), T)
             check(out[s].cpu().numpy(), want, TC_TOL if kind == "PREFILL_TC" else F32_TOL, "f32")
+
+
+@pytest.mark.parametrize("tokens,start,kind", [(1, 900, "DECODE_SPLIT"), (5, 900, "DECODE_SPLIT"), (1, 6, "DECODE_SPLIT"),
+                                               (100, 1500, "PREFILL_TC"), (300, 0, "PREFILL_TC"), (3, 50, "GENERAL")])
+@pytest.mark.parametrize("d", [64, 128])
+def test_graph_behind_other_work(cuda_lib, tokens, start, kind, d):
+    """Append, attention and read-back as a captured graph, replayed on a cleared workspace behind queued work: every launch
+    waits for what the one before it wrote, and a replay takes the inputs that stand there then."""
+    import alpaca_b200 as ab
+    rng = np.random.default_rng(41 + tokens + d)
+    S, H, Hkv, n = 3, 6, 2, start + tokens
+    parts = _kv4.random_cache(rng, S, Hkv, -(-n // 16) * 16, d)
+    cache = to_gpu(parts)
+    q, k, v = (torch.empty((S, tokens, h, d), device="cuda") for h in (H, Hkv, Hkv))
+    rot, out = torch.empty_like(q), torch.empty_like(q)
+    ko, vo = torch.empty((S, n, Hkv, d), device="cuda"), torch.empty((S, n, Hkv, d), device="cuda")
+    desc = ab.make_kv4_attn_desc(rot, cache, out, start_position=start)
+    ws = torch.zeros(max(16, ab.kv4_workspace_bytes(desc, ab.Kernel[kind])), dtype=torch.uint8, device="cuda")
+    busy = torch.zeros(1 << 26, device="cuda")
+
+    def step():
+        ab.qkv_append(q, k, v, rot, cache, start_position=start, theta=1e4)
+        ab.kv4_attention(rot, cache, out, start_position=start, kind=ab.Kernel[kind], workspace=ws)
+        ab.kv4_read(cache, ko, vo)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for x in (q, k, v):
+            x.zero_()
+        step()
+        graph = torch.cuda.CUDAGraph()
+        stream.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            step()
+        for _ in range(2):
+            for x in (q, k, v):
+                x.copy_(torch.from_numpy(rng.standard_normal(tuple(x.shape)).astype(np.float32)))
+            ws.zero_()
+            for x in (out, ko, vo):
+                x.fill_(7.0)
+            stream.synchronize()
+            for _ in range(4):
+                busy.mul_(1.0)
+            graph.replay()
+            stream.synchronize()
+            ab.device_status(stream)
+            kd, vd = ko.double().cpu().numpy(), vo.double().cpu().numpy()
+            want_v = _kv4.values(*parts[2:])[:, :, :n].swapaxes(1, 2).copy()
+            want_v[:, start:] = _kv4.values(*_kv4.quantise(v.cpu().numpy()))
+            assert np.array_equal(vd, want_v)
+            for s in range(S):
+                want = _kv4.attention(rot[s].cpu().numpy(), kd[s].swapaxes(0, 1), vd[s].swapaxes(0, 1), n)
+                check(out[s].cpu().numpy(), want, TC_TOL if kind == "PREFILL_TC" else F32_TOL, "f32")
+    del graph
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_varlen_behind_other_work(cuda_lib, d):
+    """The ragged form on a cleared workspace behind queued work."""
+    import alpaca_b200 as ab
+    rng = np.random.default_rng(43 + d)
+    H, Hkv, lens, starts = 6, 2, [100, 1, 300], [700, 50, 0]
+    parts = _kv4.random_cache(rng, 3, Hkv, 800, d)
+    cache = to_gpu(parts)
+    q = rng.standard_normal((sum(lens), H, d)).astype(np.float32)
+    offs = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    qd, od, sd = dev(q), dev(offs), dev(np.array(starts, np.int32))
+    out = torch.full(q.shape, 7.0, device="cuda")
+    desc = ab.make_kv4_varlen_desc(qd, cache, out, od, sd, max_tokens=300, max_ctx_len=800)
+    ws = torch.zeros(ab.kv4_workspace_bytes(desc), dtype=torch.uint8, device="cuda")
+    busy = torch.zeros(1 << 26, device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(4):
+        busy.mul_(1.0)
+    ab.kv4_attention_launch(desc, ws)
+    ab.device_status()
+    k, v = _kv4.values(*parts[:2]), _kv4.values(*parts[2:])
+    for s, (n, p) in enumerate(zip(lens, starts)):
+        want = _kv4.attention(q[offs[s]:offs[s + 1]], k[s], v[s], n + p)
+        check(out[offs[s]:offs[s + 1]].cpu().numpy(), want, TC_TOL, "f32")
