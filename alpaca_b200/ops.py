@@ -375,6 +375,14 @@ def _stream_handle(stream: torch.cuda.Stream | None) -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
+def _one_device(who: str, *tensors: torch.Tensor | None) -> None:
+    """The kernels follow raw addresses: every tensor of a call has to live on one CUDA device."""
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) != 1 or next(iter(devices)).type != "cuda":
+        raise AlpacaCUDAError(Status.INVALID_ARGUMENT, f"{who}: tensors must be on one CUDA device, got "
+                                                       f"{sorted(str(x) for x in devices)}")
+
+
 class Kv4Cache(NamedTuple):
     """One layer's 4-bit KV cache (alpaca_kv4_cache): codes uint8 [units, kv_heads, rows, head_dim / 2] and scales int16
     [units, kv_heads, rows, head_dim / 32] of K and V. A unit is one sequence's cache, or a block of a pool."""
@@ -507,6 +515,8 @@ def qkv_append(q: torch.Tensor | None, k: torch.Tensor | None, v: torch.Tensor |
     """Enqueue head norms + RoPE + KV append in one pass (make_qkv_desc)."""
     d_ = make_qkv_desc(q, k, v, q_out, cache, theta=theta, start_position=start_position, positions=positions,
                        interleaved=interleaved, q_norm=q_norm, k_norm=k_norm, eps=eps, block_table=block_table)
+    _one_device("qkv", q, k, v, q_out if q is not None else None, *(cache if k is not None else ()), positions, q_norm, k_norm,
+                block_table)
     qkv_launch(d_, stream)
     return d_
 
@@ -543,6 +553,7 @@ def kv4_read(cache: Kv4Cache, k_out: torch.Tensor, v_out: torch.Tensor, *, start
              stream: torch.cuda.Stream | None = None) -> Kv4ReadDesc:
     """Enqueue the read-back of 4-bit cache rows as values (make_kv4_read_desc)."""
     d_ = make_kv4_read_desc(cache, k_out, v_out, start_row=start_row, row_starts=row_starts, block_table=block_table)
+    _one_device("kv4_read", *cache, k_out, v_out, row_starts, block_table)
     kv4_read_launch(d_, stream)
     return d_
 
@@ -624,6 +635,7 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, out: torch.Tensor, *, start_
     or the one given is smaller than the library asks for (callers on a hot loop pass their own)."""
     desc = make_kv4_attn_desc(q, cache, out, start_position=start_position, ctx_lens=ctx_lens, max_ctx_len=max_ctx_len,
                               scale=scale, block_table=block_table)
+    _one_device("kv4_attention", q, out, *cache, ctx_lens, block_table, workspace)
     _kv4_run(desc, kind, workspace, q.device, stream)
     return desc
 
@@ -635,6 +647,7 @@ def kv4_prefill_varlen(q: torch.Tensor, cache: Kv4Cache, out: torch.Tensor, q_of
     """Enqueue a ragged prefill over 4-bit caches (make_kv4_varlen_desc); workspace as for kv4_attention."""
     desc = make_kv4_varlen_desc(q, cache, out, q_offsets, start_positions, max_tokens=max_tokens, max_ctx_len=max_ctx_len,
                                 scale=scale, block_table=block_table)
+    _one_device("kv4_prefill_varlen", q, out, *cache, q_offsets, start_positions, block_table, workspace)
     _kv4_run(desc, Kernel.AUTO, workspace, q.device, stream)
     return desc
 

@@ -241,3 +241,20 @@ def test_workspace_too_small_is_refused(lib):
         assert lib.alpaca_kv4_attention(ctypes.byref(d), 0, ws, n, None) == ab.Status.WORKSPACE_TOO_SMALL
     assert lib.alpaca_kv4_attention(ctypes.byref(d), 0, FAKE + 4, need, None) == ab.Status.INVALID_ARGUMENT
     assert ab.kv4_workspace_bytes(d, ab.Kernel.GENERAL) == 0
+
+
+def test_host_tensors_are_refused(lib):
+    """The kernels follow raw addresses, so a call with a host tensor must not reach them."""
+    import torch
+
+    import alpaca_b200 as ab
+    cache = ab.kv4_cache(2, 32, 2, 64, device="cpu")
+    q, k = torch.zeros((2, 3, 4, 64)), torch.zeros((2, 3, 2, 64))
+    for call in (lambda: ab.qkv_append(q, k, k.clone(), torch.empty_like(q), cache, theta=1e4),
+                 lambda: ab.qkv_append(q, None, None, torch.empty_like(q), None, theta=1e4),
+                 lambda: ab.qkv_append(None, k, k.clone(), None, (torch.empty(2, 8, 2, 64), torch.empty(2, 8, 2, 64)), theta=1e4),
+                 lambda: ab.kv4_read(cache, k, k.clone()),
+                 lambda: ab.kv4_attention(q, cache, torch.empty_like(q))):
+        with pytest.raises(ab.AlpacaCUDAError, match="one CUDA device") as e:
+            call()
+        assert e.value.status == ab.Status.INVALID_ARGUMENT
