@@ -951,7 +951,9 @@ SplitPlan split_plan(const alpaca_kv4_attn_desc& d) {
     // 4000 rows: 12.5 against 11.1).
     const int cta_tiles = p.units >= 96 ? 4 : (p.units >= 32 ? 2 : 1);
     p.cta_units = p.units <= kSms && tiles <= cta_tiles * split_warps(p.nt);
-    p.warps = p.cta_units ? std::min(tiles, split_warps(p.nt)) : split_warps(p.nt);
+    // Warps without a tile still share the join's output elements: with one warp three units' contexts of 53 rows (9/3 heads,
+    // d = 64) took 6.3 us, with eight 3.5; 16/2 heads 11.6 and 5.0.
+    p.warps = p.cta_units ? std::min(std::max(tiles, std::min(8, 2 * p.rows_per_unit())), split_warps(p.nt)) : split_warps(p.nt);
     p.ctas = p.cta_units ? static_cast<int>(p.units) : std::min(p.chunks, kSms);
     p.combine = !p.cta_units && tiles > 1;
     return p;
