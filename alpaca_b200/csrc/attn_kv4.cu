@@ -726,21 +726,46 @@ __global__ void __launch_bounds__(32 * split_warps(NT), 1) kv4_split_kernel(cons
         }
         if constexpr (kCta) {
             __syncthreads();
+            // Join: a warp per row turns the parts' maxima and sums into factors, then every thread adds four channels.
             const int warps = min(step, max(row_end > 0 ? (row_end + Ge::TK - 1) / Ge::TK : 0, 1));  // those with tiles
-            for (int i = threadIdx.x; i < QR * D; i += blockDim.x) {
-                const int row = i / D, col = i - row * D, rr = r0 + row;
+            const float* rec = reinterpret_cast<const float*>(smem);
+            float* s_f = reinterpret_cast<float*>(smem) + step * QR * Ge::REC;  // [row][warp], the sum in place 16
+            static_assert(sizeof(float) * QR * (Ge::REC + 17) <= Ge::WARP, "a warp's record and factors must fit its ring");
+            static_assert(split_warps(NT) <= 16, "a row's factors have 16 places");
+            for (int row = warp; row < QR; row += step) {
+                const float* p = rec + (lane < warps ? lane : 0) * QR * Ge::REC + row * Ge::REC + D;
+                const float m = lane < warps ? p[0] : -INFINITY;
+                float M = m;
+#pragma unroll
+                for (int o = 8; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+                const float f = m == -INFINITY ? 1.f : ex2_approx(m - M);  // without a maximum: zeros, or NaN
+                float l = lane < warps ? p[1] * f : 0.f;
+#pragma unroll
+                for (int o = 8; o >= 1; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+                if (lane < 16) s_f[row * 17 + lane] = f;
+                if (lane == 0) s_f[row * 17 + 16] = l;
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < QR * (D / 4); i += blockDim.x) {
+                const int row = i / (D / 4), col = 4 * (i - row * (D / 4)), rr = r0 + row;
                 if (rr >= a.q_rows) break;
-                const float* rec = reinterpret_cast<const float*>(smem) + row * Ge::REC;
-                float M = -INFINITY;
-                for (int k = 0; k < warps; k++) M = fmaxf(M, rec[k * QR * Ge::REC + D]);
-                float o = 0.f, l = 0.f;
+                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
                 for (int k = 0; k < warps; k++) {
-                    const float* p = rec + k * QR * Ge::REC;
-                    const float f = p[D] == -INFINITY ? 1.f : ex2_approx(p[D] - M);  // without a maximum: zeros, or NaN
-                    l = fmaf(p[D + 1], f, l);
-                    o = fmaf(p[col], f, o);
+                    const float4 v = *reinterpret_cast<const float4*>(rec + (k * QR + row) * Ge::REC + col);
+                    const float f = s_f[row * 17 + k];
+                    o.x = fmaf(v.x, f, o.x);
+                    o.y = fmaf(v.y, f, o.y);
+                    o.z = fmaf(v.z, f, o.z);
+                    o.w = fmaf(v.w, f, o.w);
                 }
-                store_out(a, seq, rr / a.group, kvh * a.group + rr % a.group, D, col, l == 0.f ? 0.f : o / l);
+                const float l = s_f[row * 17 + 16], inv = l == 0.f ? 0.f : 1.f / l;
+                if (l == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);
+                const int64_t out = seq * a.out_seq_stride + (rr / a.group) * a.out_token_stride +
+                                    static_cast<int64_t>(kvh * a.group + rr % a.group) * D + col;
+                if (a.out_f16)
+                    *reinterpret_cast<uint2*>(static_cast<__half*>(a.out) + out) = make_uint2(pack_half2(o.x * inv, o.y * inv), pack_half2(o.z * inv, o.w * inv));
+                else
+                    *reinterpret_cast<float4*>(static_cast<float*>(a.out) + out) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
             }
             return;
         }
@@ -946,13 +971,13 @@ SplitPlan split_plan(const alpaca_kv4_attn_desc& d) {
     const int tk = 4096 / d.head_dim, tiles = std::max(1, (max_context(d) + tk - 1) / tk);
     p.chunks = static_cast<int>(std::min<int64_t>(p.units * (kUnitCost + tiles), static_cast<int64_t>(kSms) * split_warps(p.nt)));
     // Few units of short contexts: one CTA per unit, one launch. With one tile a warp that wins always (9/3 heads, 517 rows:
-    // 4.8 us against 5.6); with more, only where the units fill the machine: two from 32 units on (48 units of 2000 rows: 8.2
+    // 4.3 us against 5.6); with more, only where the units fill the machine: two from 32 units on (48 units of 2000 rows: 8.2
     // against 9.3; 12 units: 8.2 against 7.7), four from 96 on (128 units of 2000 rows at d = 128: 13.9 against 16.3; 48 units of
     // 4000 rows: 12.5 against 11.1).
     const int cta_tiles = p.units >= 96 ? 4 : (p.units >= 32 ? 2 : 1);
     p.cta_units = p.units <= kSms && tiles <= cta_tiles * split_warps(p.nt);
     // Warps without a tile still share the join's output elements: with one warp three units' contexts of 53 rows (9/3 heads,
-    // d = 64) took 6.3 us, with eight 3.5; 16/2 heads 11.6 and 5.0.
+    // d = 64) took 6.2 us, with eight 3.4; 16/2 heads 11.5 and 4.4.
     p.warps = p.cta_units ? std::min(std::max(tiles, std::min(8, 2 * p.rows_per_unit())), split_warps(p.nt)) : split_warps(p.nt);
     p.ctas = p.cta_units ? static_cast<int>(p.units) : std::min(p.chunks, kSms);
     p.combine = !p.cta_units && tiles > 1;
