@@ -19,9 +19,9 @@
 //
 // What bounds it: a row of 64 channels is 72 bytes of K and V, so HBM would allow 50 cycles of an SM per 16 keys (199 issue
 // slots); decoding and both products take about 150 (d = 64, one query row) to 190. Measured on one B200: 64 sequences of
-// 1..8192 rows at 32/32 heads, d = 64, 124-139 us a call, 4.4-4.9 TB/s, 66-75% of the copy bandwidth, 0.66 instructions a
-// cycle, no pipe above 50%; 48 sequences of 1..16000 rows at 32/8 heads, d = 128, paged, 107-114 us, 59-63%. Short calls are
-// latency: 64 sequences of 1..4096 rows at 9/3 heads 15 us (floor 4.4), one session of 517 rows 4.4.
+// 1..8192 rows at 32/32 heads, d = 64, 123-139 us a call, 4.4-4.9 TB/s, 66-75% of the copy bandwidth, 0.66 instructions a
+// cycle, no pipe above 50%; 48 sequences of 1..16000 rows at 32/8 heads, d = 128, paged, 102-115 us, 59-67%. Short calls are
+// latency: 64 sequences of 1..4096 rows at 9/3 heads 15 us (floor 4.4), one session of 517 rows 4.3.
 //
 // Scores are in log2 units. A row whose context is empty, or a token that sees no row, gives zeros.
 #include <algorithm>
