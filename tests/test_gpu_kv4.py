@@ -610,3 +610,48 @@ def test_varlen_behind_other_work(cuda_lib, d):
     for s, (n, p) in enumerate(zip(lens, starts)):
         want = _kv4.attention(q[offs[s]:offs[s + 1]], k[s], v[s], n + p)
         check(out[offs[s]:offs[s + 1]].cpu().numpy(), want, TC_TOL, "f32")
+
+
+@pytest.mark.parametrize("d,H,Hkv", [(64, 2, 1), (64, 9, 3), (96, 2, 1), (128, 3, 1)])
+@pytest.mark.parametrize("S,T", [(1, 1003), (3, 739), (1, 4099), (2, 2501)])
+@pytest.mark.parametrize("by_positions", [False, True])
+def test_append_prompts_equal_definition_bitwise(cuda_lib, d, H, Hkv, S, T, by_positions):
+    """Prompts long enough for every number of tokens per CTA, none of them a divisor of the prompt."""
+    import alpaca_b200 as ab
+    rng = np.random.default_rng(S * T + d)
+    theta, starts = 10000.0, ([5, 130, 0][:S] if by_positions else [21] * S)
+    q, k, v = (rng.standard_normal((S, T, h, d)).astype(np.float32) for h in (H, Hkv, Hkv))
+    cache = ab.kv4_cache(S, max(starts) + T, Hkv, d)
+    out = torch.empty((S, T, H, d), dtype=torch.float32, device="cuda")
+    where = dict(positions=dev(np.array(starts, np.int32))) if by_positions else dict(start_position=21)
+    ab.qkv_append(dev(q), dev(k), dev(v), out, cache, theta=theta, **where)
+    ab.device_status()
+    for s, p in enumerate(starts):
+        assert np.array_equal(out[s].cpu().numpy(), oracle.rope(q[s], p, theta, True))
+        for i, x in ((0, oracle.rope(k[s], p, theta, True)), (2, v[s])):
+            codes, scales = _kv4.quantise(np.swapaxes(x, 0, 1))
+            assert np.array_equal(cache[i][s, :, p:p + T].cpu().numpy(), codes)
+            assert np.array_equal(cache[i + 1][s, :, p:p + T].cpu().numpy(), scales)
+        assert not cache.k_codes[s, :, :p].any() and not cache.k_codes[s, :, p + T:].any()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("T,H,Hkv", [(1, 4, 4), (1, 6, 2), (1, 16, 2), (2, 9, 3), (7, 9, 3), (18, 9, 3)])
+@pytest.mark.parametrize("ctx", [1, 20, 31, 65, 300, 1000])
+def test_attention_of_few_units(cuda_lib, d, T, H, Hkv, ctx):
+    """One CTA per unit: fewer tiles than warps, more, and a last group of query rows that is not full; f16 and f32 out."""
+    import alpaca_b200 as ab
+    if T > ctx:
+        ctx += T
+    rng = np.random.default_rng(ctx + T + H)
+    S = 2
+    parts = _kv4.random_cache(rng, S, Hkv, -(-ctx // 16) * 16, d)
+    q = rng.standard_normal((S, T, H, d)).astype(np.float32)
+    lens = np.array([ctx, max(0, ctx - 3)], np.int32)
+    cache, k, v = to_gpu(parts), _kv4.values(*parts[:2]), _kv4.values(*parts[2:])
+    for out_type in ("f32", "f16"):
+        out = torch.full(q.shape, 7.0, dtype=DT[out_type], device="cuda")
+        ab.kv4_attention(dev(q), cache, out, ctx_lens=dev(lens), max_ctx_len=ctx, kind=ab.Kernel.DECODE_SPLIT)
+        ab.device_status()
+        for s in range(S):
+            check(out[s].float().cpu().numpy(), _kv4.attention(q[s], k[s], v[s], int(lens[s])), F32_TOL, out_type)
