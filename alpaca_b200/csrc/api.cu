@@ -2,7 +2,6 @@
 // KernelEncoder.attention (Sources/AlpacaMetal/Backend/KernelEncoder.swift:306-343), workspace sizing
 // (KernelEncoder.decodeScratchBytes, :88-92), status codes mirroring MetalError (MetalContext.swift:7-31) and
 // the per-stream device error words that bounded device-side waits and contract checks report into.
-#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstdlib>
@@ -513,32 +512,11 @@ alpaca_cuda_status validate_kv4_attn(const alpaca_kv4_attn_desc* dp) {
 
 bool kv4_fast_head_dim(const alpaca_kv4_attn_desc& d) { return d.head_dim == 64 || d.head_dim == 128; }
 
-// Estimated times (us) of the two forms that can serve a few or more tokens at a uniform position, fitted to measurements on a
-// B200. The split kernel's grows with its tiles: query groups of 16 rows x KV heads x tiles of the context. The prefill form
-// decodes the context first and its time hardly depends on the tokens below 128 (its tiles are 128 queries high): it walks the
-// KV blocks that a work item's part has, and merges the parts where there are several. Measured split / prefill, fitted in
-// brackets: 9/3 heads at d = 64, 4000 rows: 64 tokens 16.1 / 20.4 (16.0 / 19.8), 128 tokens 20.6 / 21.4; 32/32 heads, 4 x 4000
-// rows: 16 tokens 30 / 76 (30 / 73), 64 tokens 88 / 76; 32/8 heads at d = 128, 4 x 4000 rows: 16 tokens 50 / 81 (51 / 78), 32
-// tokens 91 / 81. The split kernel's results have f32 accuracy besides.
-double kv4_split_us(const alpaca_kv4_attn_desc& d) {
-    const double group = static_cast<double>(d.n_heads / d.n_kv_heads), ctx = static_cast<double>(d.start_position) + d.tokens;
-    const double tiles = std::ceil(d.tokens * group / 16.0) * d.n_seqs * d.n_kv_heads * std::ceil(ctx * d.head_dim / 4096.0);
-    return (d.head_dim == 64 ? 10.6 : 13.0) + 2.4e-3 * tiles;
-}
-double kv4_prefill_us(const alpaca_kv4_attn_desc& d) {
-    constexpr double sms = 148;
-    const double ctx = static_cast<double>(d.start_position) + d.tokens, blocks = std::ceil(ctx / (d.head_dim == 64 ? 128.0 : 64.0));
-    const double items = static_cast<double>(d.n_seqs) * d.n_heads * std::ceil(d.tokens / 256.0);
-    const double parts = std::max(1.0, std::min({8.0, std::floor(sms / items), std::floor(blocks / 4.0)}));
-    const double walk = std::ceil(blocks / parts) * std::ceil(items * parts / sms);
-    return 5.0 + (d.head_dim == 64 ? 2.2 : 1.15) * walk + (parts > 1 ? 6.0 : 0.0);
-}
-
 alpaca_attn_kernel kv4_select(const alpaca_kv4_attn_desc& d) {
     if (d.flags & ALPACA_ATTN_FLAG_VARLEN) return ALPACA_ATTN_PREFILL_TC;
     if (!kv4_fast_head_dim(d)) return ALPACA_ATTN_GENERAL;
     if (d.ctx_lens || d.tokens < kPrefillMinTokens) return ALPACA_ATTN_DECODE_SPLIT;
-    return kv4_split_us(d) <= kv4_prefill_us(d) ? ALPACA_ATTN_DECODE_SPLIT : ALPACA_ATTN_PREFILL_TC;
+    return kv4_split_faster(d) ? ALPACA_ATTN_DECODE_SPLIT : ALPACA_ATTN_PREFILL_TC;
 }
 
 // Descriptor checks, then the kernel choice (ALPACA_ATTN_AUTO resolved) and its limits.

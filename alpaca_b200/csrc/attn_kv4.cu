@@ -1076,6 +1076,29 @@ ChunkPlan chunk_plan(const alpaca_kv4_attn_desc& d, void* ws) {
 
 }  // namespace
 
+// Estimated times (us) of the two forms, fitted to 218 calls on a B200 (8..200 tokens, 1..4 sequences, contexts up to 6200, six
+// head counts each at d = 64 and 128); over 118 others the choice averages 1.0% above the better form, 22% at worst. The split
+// kernel walks units x tiles with all warps, or (one CTA per unit) eight tiles at a time. The prefill form decodes the context
+// (bytes of f16), walks the KV blocks of a work item's part and, where there are several parts, writes and merges their records.
+// Measured split / prefill: 9/3 heads at d = 64, 4000 rows: 64 tokens 16.1 / 20.4, 128 tokens 20.6 / 21.4; 32/32 heads,
+// 4 x 4000 rows: 16 tokens 30 / 76, 64 tokens 88 / 76; 32/8 heads at d = 128, 4 x 4000 rows: 16 tokens 50 / 81, 32 tokens
+// 91 / 81. The split kernel's results have f32 accuracy besides.
+bool kv4_split_faster(const alpaca_kv4_attn_desc& d) {
+    const bool d64 = d.head_dim == 64;
+    const SplitPlan p = split_plan(d);
+    const double ctx = static_cast<double>(d.start_position) + d.tokens, tiles = std::ceil(ctx * d.head_dim / 4096.0);
+    const double split = p.cta_units ? (d64 ? 4.0 : 3.7) + (d64 ? 3.2 : 3.9) * std::ceil(tiles / 8.0)
+                                     : (d64 ? 9.8 : 11.1) + (d64 ? 2.9 : 3.4) * static_cast<double>(p.units) * tiles / (8.0 * kSms);
+    const double blocks = std::ceil(ctx / (d64 ? 128.0 : 64.0)), items = static_cast<double>(d.n_seqs) * d.n_heads * std::ceil(d.tokens / 256.0);
+    const double parts = std::max(1.0, std::min({8.0, std::floor(kSms / items), std::floor(blocks / 4.0)}));
+    const double walk = std::ceil(blocks / parts) * std::ceil(items * parts / kSms);
+    const double cache_mb = 4e-6 * d.n_seqs * ctx * d.n_kv_heads * d.head_dim;
+    const double record_mb = 8e-6 * d.n_seqs * d.n_heads * static_cast<double>(d.tokens) * d.head_dim * parts;
+    const double prefill = (d64 ? 6.2 : 6.8) + (d64 ? 1.24 : 1.0) * walk + (d64 ? 0.235 : 0.18) * cache_mb +
+                           (parts > 1.0 ? (d64 ? 4.8 : 6.2) + (d64 ? 0.65 : 0.37) * record_mb : 0.0);
+    return split <= prefill;
+}
+
 size_t kv4_workspace_bytes(const alpaca_kv4_attn_desc& d, alpaca_attn_kernel kind) {
     if (kind == ALPACA_ATTN_DECODE_SPLIT) {
         const SplitPlan p = split_plan(d);

@@ -57,6 +57,7 @@ cudaError_t launch_qkv_append(const alpaca_qkv_desc& d, unsigned* err, cudaStrea
 // start_positions / q_offsets: a ragged prefill's (each sequence's visible rows only), or null
 cudaError_t launch_kv4_read(const alpaca_kv4_read_desc& d, const int* start_positions, const int* q_offsets, unsigned* err,
                             cudaStream_t s);
+bool kv4_split_faster(const alpaca_kv4_attn_desc& d);  // against the prefill form, at a uniform position
 size_t kv4_workspace_bytes(const alpaca_kv4_attn_desc& d, alpaca_attn_kernel kind);
 cudaError_t launch_kv4_attention(const alpaca_kv4_attn_desc& d, alpaca_attn_kernel kind, float scale, void* ws, size_t ws_bytes,
                                  unsigned* err, int num_sms, cudaStream_t s);
