@@ -9,7 +9,7 @@
 //   rotation   as in rope_kv.cu: angle, cos and sin in double, rounded once to f32; products rounded separately
 //   write      f16 / f32 row, or the blocks' steps, zero points and codes (kv4.cuh)
 // A row moves 4 d or 2 d bytes in and 0.56 d .. 4 d out. Prompts are bounded by instruction issue and memory waits about
-// equally (8 x 2048 tokens of 32/8 heads at d = 128 with norms, f16 in, 4-bit cache: 73-82 us, 354 MB, 4.3-4.9 TB/s, 66% issue);
+// equally (8 x 2048 tokens of 32/8 heads at d = 128 with norms, f16 in, 4-bit cache: 73-78 us, 354 MB, 4.5-4.9 TB/s, 70% issue);
 // 4096 tokens of 9/3 heads at d = 64, f32 in: 5.8 us, one wave's latency; 64 tokens 2.7 us.
 //
 // kv4_read_kernel: four lanes per head row, f16 or f32 out in the [seq][row][head][d] layout of the f16 cache. It moves
