@@ -259,6 +259,15 @@ __device__ __forceinline__ void load_tile(const Kv4Args& a, const TileCopy& head
     }
 }
 
+// V headers of keys 2 pair (he) and 2 pair + 1 (ho), blocks 2 word and 2 word + 1, as Kv4Pairs.
+template <int D>
+__device__ __forceinline__ void decode_v_headers(uint32_t he, uint32_t ho, uint4* s_vd, int pair, int word) {
+    const Kv4Pair p0 = kv4_pair(__byte_perm(he, ho, 0x5410)), p1 = kv4_pair(__byte_perm(he, ho, 0x7632));
+    uint4* out = s_vd + ((pair >> 2) * Kv4Geo<D>::NB + 2 * word) * 4 + (pair & 3);  // [eight keys][block][pair of them]
+    out[0] = make_uint4(as_u32(p0.d), as_u32(p0.z), as_u32(p0.d16), as_u32(p0.z16));
+    out[4] = make_uint4(as_u32(p1.d), as_u32(p1.z), as_u32(p1.d16), as_u32(p1.z16));
+}
+
 // A tile's headers decoded once per warp: per key the (step, zero * 2^-24) of its K blocks in f32, and per pair of keys that
 // meet in a V operand register (2t, 2t + 1 of eight) the pair's Kv4Pair for each block.
 template <int D>
@@ -274,11 +283,7 @@ __device__ __forceinline__ void decode_headers(const uint8_t* stage, float4* s_k
         s_kd[lane + 32 * k] = make_float4(d.x, z.x, d.y, z.y);
     }
     const int pair = lane / WPK, word = lane % WPK;  // keys 2 pair, 2 pair + 1; blocks 2 word, 2 word + 1
-    const uint32_t he = vh[2 * pair * WPK + word], ho = vh[(2 * pair + 1) * WPK + word];
-    const Kv4Pair p0 = kv4_pair(__byte_perm(he, ho, 0x5410)), p1 = kv4_pair(__byte_perm(he, ho, 0x7632));
-    uint4* out = s_vd + ((pair >> 2) * Ge::NB + 2 * word) * 4 + (pair & 3);  // [eight keys][block][pair of them]
-    out[0] = make_uint4(as_u32(p0.d), as_u32(p0.z), as_u32(p0.d16), as_u32(p0.z16));
-    out[4] = make_uint4(as_u32(p1.d), as_u32(p1.z), as_u32(p1.d16), as_u32(p1.z16));
+    decode_v_headers<D>(vh[2 * pair * WPK + word], vh[(2 * pair + 1) * WPK + word], s_vd, pair, word);
 }
 
 // FO: with one or two query rows (and NT = 1) the columns that would stand empty serve other keys. Column pair c then is query
@@ -299,6 +304,43 @@ struct RowState {
     int lim[NT];             // visible rows
     float o[NT][D / 32][4];  // accumulators of the lane's four channels per chunk of V codes
 };
+
+// A tile with rows that only some of the unit's query rows see: p is 0 for the others, but 0 x NaN is NaN in the MMA. So value
+// blocks without a finite step (those that read as NaN) at rows from min_lim on count as zeros, and NaN is added by hand to the
+// channels of the query rows that do see them. Calls of one token, and tiles that every query row sees whole, never come here.
+template <int D, int NT, int FO>
+__device__ __forceinline__ void hide_nan_blocks(const uint8_t* st, uint4* s_vd, int row0, int min_lim, RowState<D, NT, FO>& s, int lane) {
+    using Ge = Kv4Geo<D>;
+    constexpr int WPK = Ge::NB / 2;
+    const uint16_t* vh = reinterpret_cast<const uint16_t*>(st + 2 * Ge::CB + Ge::HB);
+    const auto no_step = [](uint32_t h) { return (h & 0x7C00u) == 0x7C00u; };
+    const int pair = lane / WPK, word = lane % WPK;  // the headers that this lane decodes
+    uint32_t h[2];
+    bool found = false;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int row = 2 * pair + k;
+        h[k] = reinterpret_cast<const uint32_t*>(vh)[row * WPK + word];
+        if (row0 + row < min_lim) continue;
+        const uint32_t clear = (no_step(h[k]) ? 0xFFFFu : 0u) | (no_step(h[k] >> 16) ? 0xFFFF0000u : 0u);
+        h[k] &= ~clear;
+        found |= clear != 0;
+    }
+    if (!__any_sync(0xffffffffu, found)) return;
+    decode_v_headers<D>(h[0], h[1], s_vd, pair, word);
+    const int block = Ge::v_block(lane >> 2);
+    for (int row = max(min_lim - row0, 0); row < Ge::TK; row++) {
+        if (!no_step(vh[row * Ge::NB + block])) continue;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+            if (row0 + row < s.lim[nt]) {
+#pragma unroll
+                for (int c = 0; c < Ge::CPR; c++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s.o[nt][c][e] = __int_as_float(0x7FFFFFFF);
+            }
+    }
+}
 
 template <int D, int NT, int FO>
 __device__ __forceinline__ void compute_tile(const uint8_t* st, const float4* s_kd, const uint4* s_vd, int row0, int min_lim,
@@ -618,7 +660,9 @@ __device__ __forceinline__ void load_queries(const Kv4Args& a, int seq, int kvh,
 __host__ __device__ constexpr int split_warps(int NT) { return NT == 4 ? 8 : (NT == 2 ? 12 : 16); }
 
 // kCta: one CTA per unit; its warps share the unit's tiles and meet in shared memory (no records).
-template <int D, int NT, int FO, bool kCta>
+// kMany: for calls of several tokens, whose query rows see different rows of a tile. The one-token calls of up to four query
+// rows have a form without that code (paged, d = 128: 106.0 us against 108.0; one session 4.30 against 4.35).
+template <int D, int NT, int FO, bool kCta, bool kMany>
 __global__ void __launch_bounds__(32 * split_warps(NT), 1) kv4_split_kernel(const __grid_constant__ Kv4Args a) {
     using Ge = Kv4Geo<D>;
     constexpr int QR = query_rows<NT, FO>();
@@ -676,6 +720,10 @@ __global__ void __launch_bounds__(32 * split_warps(NT), 1) kv4_split_kernel(cons
             cp_async_commit();
             const uint8_t* st = ring + stage * Ge::STAGE;
             decode_headers<D>(st, s_kd, s_vd, lane);
+            if constexpr (kMany) {
+                const int row0 = (t0 + it * step) * Ge::TK;
+                if (a.tokens > 1 && row0 + Ge::TK > min_lim) hide_nan_blocks<D, NT, FO>(st, s_vd, row0, min_lim, s, lane);
+            }
             __syncwarp();
             compute_tile<D, NT, FO>(st, s_kd, s_vd, (t0 + it * step) * Ge::TK, min_lim, s, lane);
             stage = stage + 1 == kStages ? 0 : stage + 1;
@@ -999,10 +1047,10 @@ cudaLaunchConfig_t pdl_config(dim3 grid, int threads, size_t smem, cudaStream_t 
     return cfg;
 }
 
-template <int D, int NT, int FO, bool kCta>
+template <int D, int NT, int FO, bool kCta, bool kMany>
 cudaError_t launch_split_form(const Kv4Args& a, const SplitPlan& p, cudaStream_t s) {
     constexpr size_t most = split_warps(NT) * Kv4Geo<D>::WARP;
-    const auto fn = kv4_split_kernel<D, NT, FO, kCta>;
+    const auto fn = kv4_split_kernel<D, NT, FO, kCta, kMany>;
     cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          static_cast<int>(most));
     if (e != cudaSuccess) return e;
@@ -1019,7 +1067,11 @@ cudaError_t launch_split_form(const Kv4Args& a, const SplitPlan& p, cudaStream_t
 }
 template <int D, int NT, int FO>
 cudaError_t launch_split_form(const Kv4Args& a, const SplitPlan& p, cudaStream_t s) {
-    return p.cta_units ? launch_split_form<D, NT, FO, true>(a, p, s) : launch_split_form<D, NT, FO, false>(a, p, s);
+    constexpr bool one = NT == 1, many = query_rows<NT, FO>() > 1;
+    if constexpr (one && many)
+        if (a.tokens > 1)
+            return p.cta_units ? launch_split_form<D, NT, FO, true, true>(a, p, s) : launch_split_form<D, NT, FO, false, true>(a, p, s);
+    return p.cta_units ? launch_split_form<D, NT, FO, true, !one>(a, p, s) : launch_split_form<D, NT, FO, false, !one>(a, p, s);
 }
 
 template <int D>

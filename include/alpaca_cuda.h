@@ -428,7 +428,10 @@ alpaca_cuda_status alpaca_kv4_read(const alpaca_kv4_read_desc* desc, alpaca_stre
  * accuracy), PREFILL_TC (head_dim 64 / 128, uniform start_position or VARLEN: the visible rows are decoded to f16 in the
  * workspace, exactly, and the tensor-core prefill runs over them with its accuracy, P rounded to f16), GENERAL (any
  * head_dim). AUTO: PREFILL_TC for VARLEN; DECODE_SPLIT with ctx_lens; for a uniform position the one of the two that is
- * estimated faster (DECODE_SPLIT below some 32 to 128 tokens); GENERAL for other head dims. */
+ * estimated faster (DECODE_SPLIT below some 32 to 128 tokens); GENERAL for other head dims.
+ * Rows that read as NaN: DECODE_SPLIT and GENERAL give NaN to exactly the tokens that see such a row (in the block's channels for
+ * V, in the whole head for K). PREFILL_TC multiplies whole blocks of rows, hidden ones with p = 0: the outputs of the tokens that
+ * see such a row, and of up to 255 tokens of the same sequence before it, are undefined in the heads that share it. */
 typedef struct alpaca_kv4_attn_desc {
     int32_t n_seqs;          /* 1 .. 65535 */
     int32_t n_heads;
