@@ -230,9 +230,10 @@ __device__ __forceinline__ void finish_row(const AppendArgs& a, const Cta& c, in
         float ss = s2.x + s2.y;
 #pragma unroll
         for (int o = LP / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        // 1 / sqrt(mean + eps): the hardware's approximation and one Newton step
+        // 1 / sqrt(mean + eps): the hardware's approximation and one Newton step. Where the squares' sum is past f32, inf * 0 is
+        // NaN there; fmaxf drops it, and the result is 0 as 1 / sqrt(inf) is (a NaN sum stays one through y).
         const float m = fmaf(ss, a.inv_d, a.eps), y = rsqrtf(m);
-        const float inv = fmaf(y * 0.5f, fmaf(-m * y, y, 1.f), y);
+        const float inv = fmaf(y * 0.5f, fmaf(-fmaxf(m * y, 0.f), y, 1.f), y);
 #pragma unroll
         for (int s = 0; s < SETS; s++) {
             const float4* w = reinterpret_cast<const float4*>(c.s_w + (K == 0 ? 0 : d) + s * half + c0);
