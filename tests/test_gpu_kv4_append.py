@@ -1,10 +1,10 @@
-"""qkv_append: head norms at the ends of f32."""
+"""qkv_append: head norms at the ends of f32, and one token per sequence into f16 / f32 rows."""
 from __future__ import annotations
 
 import numpy as np
 import pytest
 
-from tests.test_gpu_kv4 import _norm, _rope64, dev
+from tests.test_gpu_kv4 import DT, _norm, _rope64, dev
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -30,3 +30,35 @@ def test_norm_where_the_sum_of_squares_overflows(cuda_lib, d, interleaved):
     assert not got[0, 1, 2].any() and not got[1, 4, 0].any()
     # the norm's factors and the rotation's products: a handful of f32 roundings of values up to max|.|
     assert np.max(np.abs(got - want)) <= 8 * 2.0 ** -24 * np.max(np.abs(want)) + 1e-7
+
+
+@pytest.mark.parametrize("d,H,Hkv", [(64, 9, 3), (128, 32, 8), (96, 4, 2)])
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("kind", ["f16", "f32"])
+@pytest.mark.parametrize("in_kind", ["f16", "f32"])
+def test_one_token_with_norms_into_rows(cuda_lib, d, H, Hkv, interleaved, kind, in_kind):
+    """A decode step of a model with q / k norms over the ordinary cache: every sequence at its own position; nothing but the
+    new row is written."""
+    import alpaca_b200 as ab
+    rng = np.random.default_rng(d + H)
+    S, rows, eps, theta = 37, 48, 1e-6, 10000.0
+    cast = (lambda x: x.astype(np.float16).astype(np.float32)) if in_kind == "f16" else (lambda x: x)
+    q, k, v = (cast(rng.standard_normal((S, 1, h, d)).astype(np.float32) * 2) for h in (H, Hkv, Hkv))
+    qn, kn = ((1 + 0.2 * rng.standard_normal(d)).astype(np.float32) for _ in range(2))
+    pos = rng.integers(0, rows, S).astype(np.int32)
+    pos[:2] = 0, rows - 1
+    cache = tuple(torch.full((S, rows, Hkv, d), 7.0, dtype=DT[kind], device="cuda") for _ in range(2))
+    out = torch.empty((S, 1, H, d), dtype=DT[kind], device="cuda")
+    ab.qkv_append(dev(q).to(DT[in_kind]), dev(k).to(DT[in_kind]), dev(v).to(DT[in_kind]), out, cache, theta=theta, positions=dev(pos),
+                  interleaved=interleaved, q_norm=dev(qn), k_norm=dev(kn), eps=eps)
+    ab.device_status()
+    kc, vc, qo = (x.double().cpu().numpy() for x in (*cache, out))
+    for s in range(S):
+        at = pos[s:s + 1]
+        for got, x in ((qo[s], _rope64(_norm(q[s], qn, eps), at, theta, interleaved)), (kc[s, at], _rope64(_norm(k[s], kn, eps), at, theta, interleaved)),
+                       (vc[s, at], v[s].astype(np.float64))):
+            # f32: the norm's factors and the rotation's products; f16 rounds once more
+            bound = 8 * 2.0 ** -24 * np.max(np.abs(x)) + 1e-7 + (np.abs(x) * 2.0 ** -11 if kind == "f16" else 0)
+            assert np.all(np.abs(got - x) <= bound)
+        other = np.arange(rows) != pos[s]
+        assert (kc[s, other] == 7).all() and (vc[s, other] == 7).all()
