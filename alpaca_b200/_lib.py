@@ -198,6 +198,7 @@ class QkvDesc(ctypes.Structure):
         ("flags", ctypes.c_uint32),
         ("reserved0", ctypes.c_uint32),
     ]
+    device: int | None = None  # index of the tensors' CUDA device, where the descriptor was made from tensors
 
 
 class Kv4ReadDesc(ctypes.Structure):
@@ -218,6 +219,7 @@ class Kv4ReadDesc(ctypes.Structure):
         ("flags", ctypes.c_uint32),
         ("reserved0", ctypes.c_uint32),
     ]
+    device: int | None = None  # index of the tensors' CUDA device, where the descriptor was made from tensors
 
 
 class Kv4AttnDesc(ctypes.Structure):
@@ -246,6 +248,7 @@ class Kv4AttnDesc(ctypes.Structure):
         ("start_positions", ctypes.c_void_p),
         ("cache", Kv4CacheDesc),
     ]
+    device: int | None = None  # index of the tensors' CUDA device, where the descriptor was made from tensors
 
 
 class WeightFormat(IntEnum):

@@ -375,12 +375,13 @@ def _stream_handle(stream: torch.cuda.Stream | None) -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
-def _one_device(who: str, *tensors: torch.Tensor | None) -> None:
-    """The kernels follow raw addresses: every tensor of a call has to live on one CUDA device."""
+def _one_device(who: str, *tensors: torch.Tensor | None) -> int:
+    """Index of the CUDA device that every tensor of a call has to live on: the kernels follow raw addresses."""
     devices = {t.device for t in tensors if t is not None}
     if len(devices) != 1 or next(iter(devices)).type != "cuda":
         raise AlpacaCUDAError(Status.INVALID_ARGUMENT, f"{who}: tensors must be on one CUDA device, got "
                                                        f"{sorted(str(x) for x in devices)}")
+    return next(iter(devices)).index
 
 
 class Kv4Cache(NamedTuple):
@@ -498,6 +499,8 @@ def make_qkv_desc(q: torch.Tensor | None, k: torch.Tensor | None, v: torch.Tenso
                 if kc.shape[0] != S:
                     raise AlpacaCUDAError(Status.INVALID_ARGUMENT, f"qkv: {kc.shape[0]} caches for {S} sequences")
                 d_.cache_rows, d_.cache_seq_stride = kc.shape[1], kc.stride(0) if S > 1 else 0
+    d_.device = _one_device("qkv", q, q_out if q is not None else None, k, *((v, *cache) if k is not None else ()), positions, q_norm,
+                            k_norm, block_table)
     return d_
 
 
@@ -515,8 +518,6 @@ def qkv_append(q: torch.Tensor | None, k: torch.Tensor | None, v: torch.Tensor |
     """Enqueue head norms + RoPE + KV append in one pass (make_qkv_desc)."""
     d_ = make_qkv_desc(q, k, v, q_out, cache, theta=theta, start_position=start_position, positions=positions,
                        interleaved=interleaved, q_norm=q_norm, k_norm=k_norm, eps=eps, block_table=block_table)
-    _one_device("qkv", q, k, v, q_out if q is not None else None, *(cache if k is not None else ()), positions, q_norm, k_norm,
-                block_table)
     qkv_launch(d_, stream)
     return d_
 
@@ -539,6 +540,7 @@ def make_kv4_read_desc(cache: Kv4Cache, k_out: torch.Tensor, v_out: torch.Tensor
         raise AlpacaCUDAError(Status.INVALID_ARGUMENT, f"kv4_read: cache of {heads} heads of {dim}, outputs of {H} of {D}")
     d_.k_out, d_.v_out, d_.out_row_stride = k4.data_ptr(), v4.data_ptr(), k4.stride(1)
     d_.out_seq_stride = k4.stride(0) if S > 1 else 0
+    d_.device = _one_device("kv4_read", *cache, k_out, v_out, row_starts, block_table)
     return d_
 
 
@@ -553,7 +555,6 @@ def kv4_read(cache: Kv4Cache, k_out: torch.Tensor, v_out: torch.Tensor, *, start
              stream: torch.cuda.Stream | None = None) -> Kv4ReadDesc:
     """Enqueue the read-back of 4-bit cache rows as values (make_kv4_read_desc)."""
     d_ = make_kv4_read_desc(cache, k_out, v_out, start_row=start_row, row_starts=row_starts, block_table=block_table)
-    _one_device("kv4_read", *cache, k_out, v_out, row_starts, block_table)
     kv4_read_launch(d_, stream)
     return d_
 
@@ -580,6 +581,7 @@ def make_kv4_attn_desc(q: torch.Tensor, cache: Kv4Cache, out: torch.Tensor, *, s
     d_.q, d_.q_token_stride, d_.q_seq_stride = q4.data_ptr(), q4.stride(1), q4.stride(0) if S > 1 else 0
     d_.out, d_.out_token_stride, d_.out_seq_stride = o4.data_ptr(), o4.stride(1), o4.stride(0) if S > 1 else 0
     d_.scale = float(scale)
+    d_.device = _one_device("kv4_attention", q, out, *cache, ctx_lens, block_table)
     return d_
 
 
@@ -602,6 +604,7 @@ def make_kv4_varlen_desc(q: torch.Tensor, cache: Kv4Cache, out: torch.Tensor, q_
     d_.q_dtype, d_.out_dtype = _dtype(q4), _dtype(o4)
     d_.q, d_.q_token_stride, d_.out, d_.out_token_stride = q4.data_ptr(), q4.stride(1), o4.data_ptr(), o4.stride(1)
     d_.scale = float(scale)
+    d_.device = _one_device("kv4_prefill_varlen", q, out, *cache, q_offsets, start_positions, block_table)
     return d_
 
 
@@ -620,8 +623,12 @@ def kv4_select(desc: Kv4AttnDesc) -> Kernel:
 def kv4_attention_launch(desc: Kv4AttnDesc, workspace: torch.Tensor | None = None, kind: Kernel = Kernel.AUTO,
                          stream: torch.cuda.Stream | None = None) -> None:
     """Enqueue one call of alpaca_kv4_attention on `stream` (default: torch's current stream)."""
-    ws_ptr = workspace.data_ptr() if workspace is not None else None
-    ws_len = workspace.nbytes if workspace is not None else 0
+    ws_ptr, ws_len = None, 0
+    if workspace is not None:
+        if desc.device is not None and workspace.get_device() != desc.device:
+            raise AlpacaCUDAError(Status.INVALID_ARGUMENT, f"kv4_attention: the workspace is on {workspace.device}, the call's tensors on "
+                                                           f"cuda:{desc.device}: they must be on one CUDA device")
+        ws_ptr, ws_len = workspace.data_ptr(), workspace.nbytes
     status = load().alpaca_kv4_attention(ctypes.byref(desc), kind, ws_ptr, ws_len, _stream_handle(stream))
     if status:
         check(status)
@@ -635,7 +642,6 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, out: torch.Tensor, *, start_
     or the one given is smaller than the library asks for (callers on a hot loop pass their own)."""
     desc = make_kv4_attn_desc(q, cache, out, start_position=start_position, ctx_lens=ctx_lens, max_ctx_len=max_ctx_len,
                               scale=scale, block_table=block_table)
-    _one_device("kv4_attention", q, out, *cache, ctx_lens, block_table, workspace)
     _kv4_run(desc, kind, workspace, q.device, stream)
     return desc
 
@@ -647,7 +653,6 @@ def kv4_prefill_varlen(q: torch.Tensor, cache: Kv4Cache, out: torch.Tensor, q_of
     """Enqueue a ragged prefill over 4-bit caches (make_kv4_varlen_desc); workspace as for kv4_attention."""
     desc = make_kv4_varlen_desc(q, cache, out, q_offsets, start_positions, max_tokens=max_tokens, max_ctx_len=max_ctx_len,
                                 scale=scale, block_table=block_table)
-    _one_device("kv4_prefill_varlen", q, out, *cache, q_offsets, start_positions, block_table, workspace)
     _kv4_run(desc, Kernel.AUTO, workspace, q.device, stream)
     return desc
 

@@ -1,0 +1,54 @@
+"""The 4-bit cache calls and the device that their tensors live on, without a GPU: the kernels follow raw addresses, so a
+descriptor of host tensors must not be made and a launch with a workspace elsewhere must not reach the library."""
+from __future__ import annotations
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+class Library:
+    """Stands for the loaded library: counts the calls that reach it."""
+    calls = 0
+
+    def __getattr__(self, name):
+        def call(*args):
+            Library.calls += 1
+            return 0
+        return call
+
+
+@pytest.fixture
+def library(monkeypatch):
+    from alpaca_b200 import ops
+    Library.calls = 0
+    monkeypatch.setattr(ops, "load", Library)
+    return Library
+
+
+def refused(call, match):
+    import alpaca_b200 as ab
+    with pytest.raises(ab.AlpacaCUDAError, match=match) as e:
+        call()
+    assert e.value.status == ab.Status.INVALID_ARGUMENT
+
+
+def test_descriptors_of_host_tensors_are_refused():
+    import alpaca_b200 as ab
+    cache = ab.kv4_cache(2, 32, 2, 64, device="cpu")
+    rows = tuple(torch.empty(2, 8, 2, 64) for _ in range(2))
+    q, k = torch.zeros((2, 3, 4, 64)), torch.zeros((2, 3, 2, 64))
+    for call in (lambda: ab.make_qkv_desc(q, k, k.clone(), torch.empty_like(q), cache, theta=1e4),
+                 lambda: ab.make_qkv_desc(q, None, None, torch.empty_like(q), None, theta=1e4),
+                 lambda: ab.make_qkv_desc(None, k, k.clone(), None, rows, theta=1e4),
+                 lambda: ab.make_kv4_read_desc(cache, k, k.clone()),
+                 lambda: ab.make_kv4_attn_desc(q, cache, torch.empty_like(q))):
+        refused(call, "one CUDA device")
+
+
+def test_a_workspace_elsewhere_is_refused(library):
+    import alpaca_b200 as ab
+    desc = ab.Kv4AttnDesc()
+    desc.device = 0  # as made from tensors on cuda:0
+    refused(lambda: ab.kv4_attention_launch(desc, torch.empty(64, dtype=torch.uint8)), "workspace")
+    assert library.calls == 0
