@@ -368,11 +368,15 @@ def decode_project(weights: list[torch.Tensor], fmt: str, k: int, x: torch.Tenso
 
 # ---------------------------------------------------------------------------------------------- 4-bit KV cache
 
-def _stream_handle(stream: torch.cuda.Stream | None) -> int:
-    """cudaStream_t of `stream`, or of torch's current stream (without building a Stream object: 3 us a call)."""
-    if stream is not None:
-        return stream.cuda_stream
-    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+def _stream_handle(stream: torch.cuda.Stream | None, device: int | None) -> int:
+    """cudaStream_t of `stream`, or of torch's current stream (without building a Stream object: 3 us a call). The library
+    launches on the current device: a call whose tensors (`device`, where known) or stream live on another is refused."""
+    current = torch._C._cuda_getDevice()
+    if device is not None and device != current or stream is not None and stream.device_index != current:
+        raise AlpacaCUDAError(Status.INVALID_ARGUMENT,
+                              f"tensors on cuda:{device}, " + (f"stream on cuda:{stream.device_index}, " if stream is not None else "") +
+                              f"but cuda:{current} is current: make the call under torch.cuda.device of its tensors")
+    return stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(current)
 
 
 def _one_device(who: str, *tensors: torch.Tensor | None) -> int:
@@ -505,7 +509,7 @@ def make_qkv_desc(q: torch.Tensor | None, k: torch.Tensor | None, v: torch.Tenso
 
 
 def qkv_launch(desc: QkvDesc, stream: torch.cuda.Stream | None = None) -> None:
-    status = load().alpaca_qkv_append(ctypes.byref(desc), _stream_handle(stream))
+    status = load().alpaca_qkv_append(ctypes.byref(desc), _stream_handle(stream, desc.device))
     if status:
         check(status)
 
@@ -545,7 +549,7 @@ def make_kv4_read_desc(cache: Kv4Cache, k_out: torch.Tensor, v_out: torch.Tensor
 
 
 def kv4_read_launch(desc: Kv4ReadDesc, stream: torch.cuda.Stream | None = None) -> None:
-    status = load().alpaca_kv4_read(ctypes.byref(desc), _stream_handle(stream))
+    status = load().alpaca_kv4_read(ctypes.byref(desc), _stream_handle(stream, desc.device))
     if status:
         check(status)
 
@@ -629,7 +633,7 @@ def kv4_attention_launch(desc: Kv4AttnDesc, workspace: torch.Tensor | None = Non
             raise AlpacaCUDAError(Status.INVALID_ARGUMENT, f"kv4_attention: the workspace is on {workspace.device}, the call's tensors on "
                                                            f"cuda:{desc.device}: they must be on one CUDA device")
         ws_ptr, ws_len = workspace.data_ptr(), workspace.nbytes
-    status = load().alpaca_kv4_attention(ctypes.byref(desc), kind, ws_ptr, ws_len, _stream_handle(stream))
+    status = load().alpaca_kv4_attention(ctypes.byref(desc), kind, ws_ptr, ws_len, _stream_handle(stream, desc.device))
     if status:
         check(status)
 
@@ -658,6 +662,7 @@ def kv4_prefill_varlen(q: torch.Tensor, cache: Kv4Cache, out: torch.Tensor, q_of
 
 
 def _kv4_run(desc: Kv4AttnDesc, kind: Kernel, workspace: torch.Tensor | None, device, stream) -> None:
+    _stream_handle(stream, desc.device)  # refused before anything is allocated
     need = kv4_workspace_bytes(desc, kind)
     if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
         if stream is None:

@@ -52,3 +52,45 @@ def test_a_workspace_elsewhere_is_refused(library):
     desc.device = 0  # as made from tensors on cuda:0
     refused(lambda: ab.kv4_attention_launch(desc, torch.empty(64, dtype=torch.uint8)), "workspace")
     assert library.calls == 0
+
+
+class Stream:
+    """What the launches read of a torch.cuda.Stream."""
+    def __init__(self, device):
+        self.device_index, self.cuda_stream = device, 77
+
+
+def launches():
+    import alpaca_b200 as ab
+    return [(ab.QkvDesc, ab.qkv_launch), (ab.Kv4ReadDesc, ab.kv4_read_launch),
+            (ab.Kv4AttnDesc, lambda d, stream=None: ab.kv4_attention_launch(d, stream=stream))]
+
+
+@pytest.mark.parametrize("i", range(3))
+def test_a_call_away_from_its_tensors_is_refused(library, monkeypatch, i):
+    """The library launches on the current device; the device index is stubbed."""
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 55, raising=False)
+    make, launch = launches()[i]
+    desc = make()
+    desc.device = 1
+    refused(lambda: launch(desc), "cuda:0 is current")
+    refused(lambda: launch(desc, stream=Stream(1)), "cuda:0 is current")
+    desc.device = 0
+    refused(lambda: launch(desc, stream=Stream(1)), "stream on cuda:1")
+    assert library.calls == 0
+    launch(desc)
+    launch(desc, stream=Stream(0))
+    launch(make())  # a descriptor filled by hand names no device
+    assert library.calls == 3
+
+
+def test_no_workspace_is_allocated_for_a_refused_call(library, monkeypatch):
+    from alpaca_b200 import ops
+    import alpaca_b200 as ab
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(ops, "kv4_workspace_bytes", lambda *a: 1 / 0)
+    desc = ab.Kv4AttnDesc()
+    desc.device = 1
+    refused(lambda: ops._kv4_run(desc, ab.Kernel.AUTO, None, "cuda:1", None), "cuda:0 is current")
+    assert library.calls == 0
