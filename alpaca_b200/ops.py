@@ -643,7 +643,11 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, out: torch.Tensor, *, start_
                   block_table: torch.Tensor | None = None, kind: Kernel = Kernel.AUTO, workspace: torch.Tensor | None = None,
                   stream: torch.cuda.Stream | None = None) -> Kv4AttnDesc:
     """Enqueue attention over the 4-bit cache (make_kv4_attn_desc); allocates the workspace with torch when none is given
-    or the one given is smaller than the library asks for (callers on a hot loop pass their own)."""
+    or the one given is smaller than the library asks for (callers on a hot loop pass their own).
+
+    Kernel.AUTO takes the kernel estimated faster: past some 32 to 128 tokens at one position that is PREFILL_TC, which rounds
+    the queries and P to f16 and holds the visible rows as f16 in the workspace. kind=Kernel.DECODE_SPLIT keeps f32 accuracy
+    at every token count. With `ctx_lens` every call runs on DECODE_SPLIT; prompts of different lengths: kv4_prefill_varlen."""
     desc = make_kv4_attn_desc(q, cache, out, start_position=start_position, ctx_lens=ctx_lens, max_ctx_len=max_ctx_len,
                               scale=scale, block_table=block_table)
     _kv4_run(desc, kind, workspace, q.device, stream)
@@ -654,7 +658,8 @@ def kv4_prefill_varlen(q: torch.Tensor, cache: Kv4Cache, out: torch.Tensor, q_of
                        start_positions: torch.Tensor, *, max_tokens: int, max_ctx_len: int, scale: float = 0.0,
                        block_table: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
                        stream: torch.cuda.Stream | None = None) -> Kv4AttnDesc:
-    """Enqueue a ragged prefill over 4-bit caches (make_kv4_varlen_desc); workspace as for kv4_attention."""
+    """Enqueue a ragged prefill over 4-bit caches (make_kv4_varlen_desc); workspace as for kv4_attention: it holds
+    max_ctx_len rows of every sequence as f16, whatever their contexts are."""
     desc = make_kv4_varlen_desc(q, cache, out, q_offsets, start_positions, max_tokens=max_tokens, max_ctx_len=max_ctx_len,
                                 scale=scale, block_table=block_table)
     _kv4_run(desc, Kernel.AUTO, workspace, q.device, stream)

@@ -424,11 +424,18 @@ alpaca_cuda_status alpaca_kv4_read(const alpaca_kv4_read_desc* desc, alpaca_stre
  * ctx_lens entries lie in [0, max_ctx_len]; a token that sees no row (an empty context, or ctx < tokens) gives zeros.
  * With ALPACA_ATTN_FLAG_VARLEN the call is a ragged prefill: q_offsets, start_positions, total_tokens, tokens and
  * max_ctx_len as in alpaca_attn_desc.
- * Kernels (alpaca_attn_kernel): DECODE_SPLIT (head_dim 64 / 128, any token count: a few tokens over long contexts; f32
- * accuracy), PREFILL_TC (head_dim 64 / 128, uniform start_position or VARLEN: the visible rows are decoded to f16 in the
- * workspace, exactly, and the tensor-core prefill runs over them with its accuracy, P rounded to f16), GENERAL (any
- * head_dim). AUTO: PREFILL_TC for VARLEN; DECODE_SPLIT with ctx_lens; for a uniform position the one of the two that is
- * estimated faster (DECODE_SPLIT below some 32 to 128 tokens); GENERAL for other head dims.
+ * Kernels (alpaca_attn_kernel):
+ *   DECODE_SPLIT  head_dim 64 / 128, any token count: a few tokens over long contexts. f32 accuracy. Every 16 query rows (token x
+ *                 query head of a KV head) read the cache again.
+ *   PREFILL_TC    head_dim 64 / 128, uniform start_position or VARLEN: the visible rows are decoded to f16 in the workspace,
+ *                 exactly, and the tensor-core prefill runs over them with its accuracy: queries and P rounded to f16. The
+ *                 workspace holds 4 x n_seqs x rows x n_kv_heads x head_dim bytes of them, rows = start_position + tokens, or
+ *                 max_ctx_len with VARLEN whatever the actual contexts are, next to the prefill's own.
+ *   GENERAL       any head_dim, f32 accuracy.
+ * AUTO: PREFILL_TC for VARLEN; DECODE_SPLIT with ctx_lens, at any token count (prompts of different lengths belong in a VARLEN
+ * call); for a uniform position the one of the two that is estimated faster (DECODE_SPLIT below some 32 to 128 tokens), so f32
+ * queries keep f32 accuracy below that and are rounded above it: a caller who needs it at every count names DECODE_SPLIT;
+ * GENERAL for other head dims.
  * Rows that read as NaN: DECODE_SPLIT and GENERAL give NaN to exactly the tokens that see such a row (in the block's channels for
  * V, in the whole head for K). PREFILL_TC multiplies whole blocks of rows, hidden ones with p = 0: the outputs of the tokens that
  * see such a row, and of up to 255 tokens of the same sequence before it, are undefined in the heads that share it. */
