@@ -25,6 +25,7 @@
 //
 // Scores are in log2 units. A row whose context is empty, or a token that sees no row, gives zeros.
 #include <algorithm>
+#include <climits>
 #include <cmath>
 
 #include "kv4.cuh"
@@ -557,7 +558,8 @@ __device__ __forceinline__ Chunk find_chunk(const Kv4Args& a, int64_t index, int
     for (int s0 = 0;; s0 += 32) {
         const int s = s0 + lane;
         const int L = s0 == 0 ? held[0] : (s0 == 32 ? held[1] : (s < a.n_seqs ? ctx_of(a, s) : 0));
-        const int mine = s < a.n_seqs ? unit_places<D>(L) : 0;  // at most 2^25 + 1: a block's sum fits 32 bits
+        static_assert(32 * (kUnitCost + (int64_t(1) << 30) / Kv4Geo<D>::TK) <= INT_MAX, "places of 32 sequences must fit 32 bits");
+        const int mine = s < a.n_seqs ? unit_places<D>(L) : 0;  // contexts are at most 2^30 rows
         int incl = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {

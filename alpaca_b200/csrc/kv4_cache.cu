@@ -440,7 +440,7 @@ struct ReadArgs {
     // ragged prefill: the first start_positions[s] + (q_offsets[s + 1] - q_offsets[s]) rows of each sequence (null: n_rows)
     const int* start_positions;
     const int* q_offsets;
-    int start, n_rows, n_kv_heads, d, out_f16;
+    int start, n_rows, n_kv_heads, out_f16;
     unsigned* err;
 };
 
@@ -631,7 +631,6 @@ cudaError_t launch_kv4_read(const alpaca_kv4_read_desc& d, const int* start_posi
     a.start = d.start_row;
     a.n_rows = d.n_rows;
     a.n_kv_heads = d.n_kv_heads;
-    a.d = d.head_dim;
     a.out_f16 = d.out_dtype == ALPACA_F16;
     a.err = err;
     const int64_t rows = static_cast<int64_t>(d.n_rows) * d.n_kv_heads;
