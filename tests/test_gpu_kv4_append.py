@@ -1,9 +1,11 @@
-"""qkv_append: head norms at the ends of f32, and one token per sequence into f16 / f32 rows."""
+"""qkv_append: head norms at the ends of f32, one token per sequence into f16 / f32 rows, every head_dim, RoPE bases below 1."""
 from __future__ import annotations
 
 import numpy as np
 import pytest
 
+import oracle
+from tests import _kv4
 from tests.test_gpu_kv4 import DT, _norm, _rope64, dev
 
 torch = pytest.importorskip("torch")
@@ -62,3 +64,30 @@ def test_one_token_with_norms_into_rows(cuda_lib, d, H, Hkv, interleaved, kind, 
             assert np.all(np.abs(got - x) <= bound)
         other = np.arange(rows) != pos[s]
         assert (kc[s, other] == 7).all() and (vc[s, other] == 7).all()
+
+
+@pytest.mark.parametrize("d", [32, 64, 96, 128, 160, 192, 224, 256])
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("theta", [1e4, 1.0, 0.01])
+def test_every_head_dim_bitwise(cuda_lib, d, interleaved, theta):
+    """Queries as the oracle rotates them and cache rows as the format defines them, bit for bit; a base below 1 turns faster
+    with the channel, up to 2^33 radians here."""
+    import alpaca_b200 as ab
+    rng = np.random.default_rng(d)
+    for start in (0, 1_000_003, 1 << 30 if theta >= 1 else 1 << 27):
+        T = 7 if start < 1 << 30 else 1
+        start -= T if start else 0
+        q = rng.standard_normal((1, T, 3, d)).astype(np.float32)
+        out = torch.empty(q.shape, device="cuda")
+        ab.qkv_append(dev(q), None, None, out, None, theta=theta, start_position=start, interleaved=interleaved)
+        ab.device_status()
+        assert np.array_equal(out[0].cpu().numpy(), oracle.rope(q[0], start, theta, interleaved))
+    k, v = (rng.standard_normal((2, 7, 3, d)).astype(np.float32) for _ in range(2))
+    cache = ab.kv4_cache(2, 32, 3, d)
+    ab.qkv_append(None, dev(k), dev(v), None, cache, theta=theta, start_position=20, interleaved=interleaved)
+    ab.device_status()
+    for s in range(2):
+        for i, x in ((0, oracle.rope(k[s], 20, theta, interleaved)), (2, v[s])):
+            codes, scales = _kv4.quantise(np.swapaxes(x, 0, 1))
+            assert np.array_equal(cache[i][s, :, 20:27].cpu().numpy(), codes)
+            assert np.array_equal(cache[i + 1][s, :, 20:27].cpu().numpy(), scales)
