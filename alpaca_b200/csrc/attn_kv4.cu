@@ -18,10 +18,12 @@
 //   general kernel fp32 SIMT, any head_dim that is a multiple of 32 up to 256: one warp per query row.
 //
 // What bounds it: a row of 64 channels is 72 bytes of K and V, so HBM would allow 50 cycles of an SM per 16 keys (199 issue
-// slots); decoding and both products take about 150 (d = 64, one query row) to 190. Measured on one B200: 64 sequences of
-// 1..8192 rows at 32/32 heads, d = 64, 123-139 us a call, 4.4-4.9 TB/s, 66-75% of the copy bandwidth, 0.66 instructions a
-// cycle, no pipe above 50%; 48 sequences of 1..16000 rows at 32/8 heads, d = 128, paged, 102-115 us, 59-67%. Short calls are
-// latency: 64 sequences of 1..4096 rows at 9/3 heads 15 us (floor 4.4), one session of 517 rows 4.3.
+// slots); decoding and both products take about 150 (d = 64, one query row) to 190, and issue is active 67-69% of the time: the
+// long calls are bound by the instructions they decode with at the rate that four warps a scheduler issue, not by one unit.
+// Measured on one B200: 64 sequences of 1..8192 rows at 32/32 heads, d = 64, 118-139 us a call, 4.4-5.1 TB/s, 66-78% of the copy
+// bandwidth (ALU 55%, shared-memory wavefronts 61%, FMA 42%, tensor 30%); 48 sequences of 1..16000 rows at 32/8 heads, d = 128,
+// paged, 99-115 us, 59-68%. Short calls are latency: 64 sequences of 1..4096 rows at 9/3 heads 15 us (floor 4.4), one session of
+// 517 rows 4.3.
 //
 // Scores are in log2 units. A row whose context is empty, or a token that sees no row, gives zeros.
 #include <algorithm>
@@ -658,7 +660,9 @@ __device__ __forceinline__ void load_queries(const Kv4Args& a, int seq, int kvh,
     }
 }
 
-// Warps of a CTA, one CTA per SM: as many as the registers of the form allow (128, 168 and 255 a thread).
+// Warps of a CTA, one CTA per SM: as many as the registers of the form allow (128, 168 and 255 a thread). The forms for d = 128
+// spill 4 to 96 bytes of their units' state, those for d = 64 none to 56. It is not what costs them: the paged decode's form
+// spills 64, the same with kMany 16, and that one is 2% slower.
 __host__ __device__ constexpr int split_warps(int NT) { return NT == 4 ? 8 : (NT == 2 ? 12 : 16); }
 
 // kCta: one CTA per unit; its warps share the unit's tiles and meet in shared memory (no records).
@@ -913,6 +917,11 @@ __global__ void __launch_bounds__(32 * W) kv4_combine_kernel(const __grid_consta
 }
 
 // ------------------------------------------------------------------------------------------------ general kernel
+//
+// For head dims without a form of the split kernel: f32 arithmetic, one warp per query row and no staging, so each query row
+// decodes its cache rows again, a lane's K words lie d / 2 bytes from its neighbour's, and eight lanes load one V word. Bound by
+// that latency chain, far from the bytes: 64 sequences of 1..4096 rows at 8/2 heads, d = 96, 1.44 ms (floor 4.4 us), d = 256
+// 2.6 ms; a prompt of 1024 tokens 0.58 and 1.3 ms; at d = 64 the split kernel takes 15 us where this one takes 1.2 ms.
 
 constexpr int kGenWarps = 4;
 constexpr int kGenMaxD = 256;
@@ -1130,10 +1139,12 @@ ChunkPlan chunk_plan(const alpaca_kv4_attn_desc& d, void* ws) {
 
 }  // namespace
 
-// Estimated times (us) of the two forms, fitted to 218 calls on a B200 (8..200 tokens, 1..4 sequences, contexts up to 6200, six
-// head counts each at d = 64 and 128); over 118 others the choice averages 1.0% above the better form, 22% at worst. The split
-// kernel walks units x tiles with all warps, or (one CTA per unit) eight tiles at a time. The prefill form decodes the context
-// (bytes of f16), walks the KV blocks of a work item's part and, where there are several parts, writes and merges their records.
+// Estimated times (us) of the two forms, fitted by least squares of the relative error to 218 calls on a B200 (8..200 tokens, 1..4
+// sequences, contexts up to 6200, five head counts at d = 64 and four at 128); over 208 others, timed later, the choice averages
+// 1.3% above the better form, 26% at worst (both sets: profiles/kv4_choice.csv; the split estimates are 16-19% off by themselves,
+// the prefill's 6-7%). The split kernel walks units x tiles with all warps, or (one CTA per unit) eight tiles at a time. The
+// prefill form decodes the context (bytes of f16), walks the KV blocks of a work item's part and, where there are several
+// parts, writes and merges their records.
 // Measured split / prefill: 9/3 heads at d = 64, 4000 rows: 64 tokens 16.1 / 20.4, 128 tokens 20.6 / 21.4; 32/32 heads,
 // 4 x 4000 rows: 16 tokens 30 / 76, 64 tokens 88 / 76; 32/8 heads at d = 128, 4 x 4000 rows: 16 tokens 50 / 81, 32 tokens
 // 91 / 81. The split kernel's results have f32 accuracy besides.

@@ -102,7 +102,7 @@ __device__ __forceinline__ void store8(void* p, int64_t off, int f16, const floa
     }
 }
 
-// sin and cos of x (|x| < 2^31) to about 2e-16, for one rounding to f32: the nearest multiple of pi/2 taken off in two FMAs
+// sin and cos of x (|x| < 2^50, tested to 2^33) to about 2e-16, for one rounding to f32: the nearest multiple of pi/2 taken off in two FMAs
 // against a 106-bit pi/2 (Cody and Waite's reduction), then the Taylor series on [-pi/4, pi/4] (next terms below 5e-17).
 // The call it replaces takes some 700 instructions, most of an append's work at few heads; this takes about 50.
 __device__ __forceinline__ float2 sincos_f32(double x) {  // (cos, sin)
@@ -540,9 +540,10 @@ int append_lanes(int head_dim) {
 }
 
 // Tokens per CTA: the power of two up to kAppendTokens with the least waves x time of a CTA, which is about 1.75 us (its wait,
-// its angles, its loads' latency) and 0.0057 us per lane of work (fitted, a B200 holds four CTAs an SM). Measured at 1 / 2 / 4 /
-// 8 tokens, us: 64 tokens of 32/8 heads at d = 128 2.7 / 3.5 / 5.4 / 9.0; 1024 tokens 8.8 / 9.0 / 14.8 / 20.6; 16384 tokens
-// 92 / 78 / 73 / 76; 4096 tokens of 9/3 heads at d = 64 17 / 10 / 7.1 / 5.9; 2048 tokens 9.9 / 5.5 / 4.2 / 5.4.
+// its angles, its loads' latency) and 0.0057 us per lane of work (fitted to the calls below; a B200 holds four CTAs an SM). It
+// ranks the choices; the time of a single wave it overstates up to twice. Measured at 1 / 2 / 4 / 8 tokens, us: 64 tokens of
+// 32/8 heads at d = 128 2.7 / 3.5 / 5.4 / 9.0; 1024 tokens 8.8 / 9.0 / 14.8 / 20.6; 16384 tokens 92 / 78 / 73 / 76; 4096 tokens
+// of 9/3 heads at d = 64 17 / 10 / 7.1 / 5.9; 2048 tokens 9.9 / 5.5 / 4.2 / 5.4.
 int append_tokens(const alpaca_qkv_desc& d, int row_lanes) {
     const double token_lanes = static_cast<double>(d.n_heads + 2 * d.n_kv_heads) * row_lanes;
     constexpr int64_t resident = 148 * 4;
